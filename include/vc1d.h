@@ -329,6 +329,147 @@ typedef struct vc1d_update_bwd_args {
 VC1D_API int vc1d_update_bwd(const vc1d_update_bwd_args* args, void* stream);
 VC1D_API uint32_t vc1d_sizeof_update_bwd_args(void);
 
+/*
+ * Linear attention with a fixed decay for each head: linear_attention_fn (prompts, training).  The long-range
+ * companion of the Canon convolution; the reference's attention (model/model.py:760-900) is a softmax over a growing
+ * cache, so it has no counterpart there.  With a = exp(log_decay[h]):
+ *     valid token:   S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t
+ *     masked token:  S_t = S_{t-1},                 o_t = 0      (its q, k, v are not read)
+ *     packed rows:   S starts at zero at the first token of each run of equal seq_idx
+ * States are fp32 [batch, heads, dim_k, dim_v].  heads is a multiple of heads_k and of heads_v; head h reads key head
+ * h / (heads / heads_k) and value head h / (heads / heads_v).  Head dimensions 1..VC1D_LINEAR_MAX_DIM.
+ * Sums, powers of the decay and states are fp32; out is rounded once.  In the 16-bit tensor-core kernel the products
+ * inside a chunk and the state that queries read are rounded to the I/O type before the second product.
+ */
+#define VC1D_LINEAR_MAX_DIM 256
+
+enum {
+    VC1D_LINEAR_AUTO = 0,
+    VC1D_LINEAR_SIMT = 1,  /* fp32 pipes: any strides, every type */
+    VC1D_LINEAR_MMA = 2    /* tensor cores: 16-bit types, channel stride 1, 16-byte aligned rows */
+};
+
+typedef struct vc1d_linear_args {
+    uint32_t struct_size;   /* sizeof(vc1d_linear_args) */
+    int32_t dtype;          /* q, k, v, out: VC1D_F32 | VC1D_BF16 | VC1D_F16 */
+    int32_t batch, seqlen, heads, heads_k, heads_v, dim_k, dim_v;
+    int32_t kernel;         /* VC1D_LINEAR_* */
+    const void* q;          /* [batch, seqlen, heads, dim_k] */
+    const void* k;          /* [batch, seqlen, heads_k, dim_k] */
+    const void* v;          /* [batch, seqlen, heads_v, dim_v] */
+    void* out;              /* [batch, seqlen, heads, dim_v]; must not overlap q, k, v */
+    int64_t q_strides[4], k_strides[4], v_strides[4], out_strides[4];   /* in elements; inputs may repeat (stride 0) */
+    const float* log_decay; /* [heads] */
+    const void* mask;       /* [batch, seqlen] or NULL; 0 = masked */
+    int64_t mask_strides[2];
+    const int32_t* seq_idx; /* [batch, seqlen] or NULL; not combined with mask or states (VC1D_E_SHAPE) */
+    int64_t seq_strides[2];
+    const float* initial_state; /* [batch, heads, dim_k, dim_v] or NULL (zeros) */
+    float* final_state;         /* the same, or NULL; must not overlap initial_state */
+    int64_t initial_strides[4], final_strides[4];
+    int32_t mask_dtype;
+    float scale;
+    /* Device memory for splitting the time axis where batch * heads leave SMs idle: vc1d_linear_workspace() bytes,
+     * 16-byte aligned, contents irrelevant.  NULL or too small: the axis is not split.  Launches that may overlap
+     * must not share it. */
+    void* workspace;
+    int64_t workspace_bytes;
+    int32_t segments;       /* parts of the time axis: 0 = automatic */
+    int32_t reserved;
+} vc1d_linear_args;
+
+VC1D_API int vc1d_linear(const vc1d_linear_args* args, void* stream);
+VC1D_API int64_t vc1d_linear_workspace(const vc1d_linear_args* args);  /* bytes; negative: VC1D_E_* */
+VC1D_API uint32_t vc1d_sizeof_linear_args(void);
+
+/*
+ * Backward of vc1d_linear: gradients of q, k, v and of the initial state, for the gradients of out and of the final
+ * state.  `f` describes the forward call (out, final_state, workspace and segments in it are ignored).  Gradients of
+ * shared key / value heads are summed over the heads that read them, in a fixed order.
+ */
+typedef struct vc1d_linear_bwd_args {
+    uint32_t struct_size;   /* sizeof(vc1d_linear_bwd_args) */
+    int32_t segments;       /* parts of the time axis: 0 = automatic */
+    vc1d_linear_args f;
+    const void* dout;       /* like out */
+    const float* dfinal;    /* like final_state, or NULL */
+    void *dq, *dk, *dv;     /* like q, k, v; no two of them overlap, nor any input */
+    float* dinitial;        /* like initial_state, or NULL */
+    int64_t dout_strides[4], dfinal_strides[4], dq_strides[4], dk_strides[4], dv_strides[4], dinitial_strides[4];
+    void* workspace;        /* vc1d_linear_bwd_workspace() bytes; required where it is not 0 and heads are shared */
+    int64_t workspace_bytes;
+} vc1d_linear_bwd_args;
+
+VC1D_API int vc1d_linear_bwd(const vc1d_linear_bwd_args* args, void* stream);
+VC1D_API int64_t vc1d_linear_bwd_workspace(const vc1d_linear_bwd_args* args);  /* bytes; negative: VC1D_E_* */
+VC1D_API uint32_t vc1d_sizeof_linear_bwd_args(void);
+
+/*
+ * One token of linear attention: linear_attention_update.  `state` is updated in place.  Rows of the batch whose mask
+ * is 0 (idle slots of a captured decode step) keep their state untouched and get zeros.
+ */
+typedef struct vc1d_linear_update_args {
+    uint32_t struct_size;   /* sizeof(vc1d_linear_update_args) */
+    int32_t dtype;          /* q, k, v, out */
+    int32_t batch, heads, heads_k, heads_v, dim_k, dim_v;
+    const void* q;          /* [batch, heads, dim_k] */
+    const void* k;          /* [batch, heads_k, dim_k] */
+    const void* v;          /* [batch, heads_v, dim_v] */
+    void* out;              /* [batch, heads, dim_v] */
+    float* state;           /* [batch, heads, dim_k, dim_v] */
+    const float* log_decay; /* [heads] */
+    const void* mask;       /* [batch] or NULL */
+    int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3], state_strides[4];
+    int64_t mask_stride;
+    int32_t mask_dtype;
+    float scale;
+} vc1d_linear_update_args;
+
+VC1D_API int vc1d_linear_update(const vc1d_linear_update_args* args, void* stream);
+VC1D_API uint32_t vc1d_sizeof_linear_update_args(void);
+
+/*
+ * Pages of a cache of states.  A page is row i along the first dimension of every tensor of a list (the Canon states
+ * of all layers and positions, their positions' vectors, linear attention states): what belongs to one request or
+ * beam.  One launch moves pages of all tensors in place.  All pages are read before any page that is written is
+ * visible as a source: page i afterwards holds what its source held BEFORE the call, however the moves chain or
+ * cross.  (The reference gathers one new tensor per layer and position, model/model.py:1340-1364.)
+ *   VC1D_PAGES_REORDER: source[pages]: page i takes page source[i]          (source[i] == i: left alone)
+ *   VC1D_PAGES_COPY:    src[n], dst[n]: page dst[i] takes page src[i]; of equal dst the lowest i counts
+ *   VC1D_PAGES_FREE:    dst[n]: page dst[i] is cleared to zero bytes
+ *   VC1D_PAGES_COMPACT: live[pages] (bytes, 0 = free): with n = number of live pages, the free pages below n take,
+ *                       in order, the live pages from n on; pages from n on are left as they are.  new_index[pages]
+ *                       receives where each page is afterwards (-1: it was free), count[1] receives n.
+ * A source or destination outside 0..pages-1 moves nothing (checked by the kernel).
+ */
+#define VC1D_PAGES_MAX_TENSORS 128
+#define VC1D_PAGES_MAX_PAGES 8192
+enum { VC1D_PAGES_REORDER = 0, VC1D_PAGES_COPY = 1, VC1D_PAGES_FREE = 2, VC1D_PAGES_COMPACT = 3 };
+
+typedef struct vc1d_page_tensor {
+    void* base;             /* page 0 */
+    int64_t page_bytes;     /* a page is contiguous */
+    int64_t stride_bytes;   /* from page to page, at least page_bytes */
+} vc1d_page_tensor;
+
+typedef struct vc1d_pages_args {
+    uint32_t struct_size;   /* sizeof(vc1d_pages_args) */
+    int32_t op;             /* VC1D_PAGES_* */
+    int32_t pages;          /* 0..VC1D_PAGES_MAX_PAGES */
+    int32_t n_tensors;      /* 0..VC1D_PAGES_MAX_TENSORS */
+    const vc1d_page_tensor* tensors;  /* HOST array; no two tensors overlap */
+    const void* source;     /* device: REORDER source[pages], COPY src[n] */
+    const void* dst;        /* device: COPY, FREE dst[n] */
+    const uint8_t* live;    /* device: COMPACT live[pages] */
+    int32_t* new_index;     /* device: COMPACT, [pages] */
+    int32_t* count;         /* device: COMPACT, [1] */
+    int32_t n;              /* COPY, FREE: entries */
+    int32_t index_dtype;    /* of source and dst: VC1D_I32 | VC1D_I64 */
+} vc1d_pages_args;
+
+VC1D_API int vc1d_pages(const vc1d_pages_args* args, void* stream);
+VC1D_API uint32_t vc1d_sizeof_pages_args(void);
+
 /* ABI version of the loaded library (VC1D_ABI_VERSION it was built with). */
 VC1D_API int vc1d_abi_version(void);
 
@@ -348,7 +489,7 @@ VC1D_API uint64_t vc1d_launch_count(void);
 
 /* Name of the kernel the most recent launcher call on this thread selected ("channel_last",
  * "time_major", "generic", "tma", "update_vec", "update_lane", "update_generic", "bwd_tma", "bwd_generic",
- * "update_bwd").  Per host thread: a backward pass run by an autograd worker thread does not show
+ * "update_bwd", "linear_simt", "linear_mma", "linear_update", "pages").  Per host thread: a backward pass run by an autograd worker thread does not show
  * up in the thread that called the forward. */
 VC1D_API const char* vc1d_last_kernel(void);
 

@@ -8,6 +8,11 @@ Public surface:
   causal_conv1d_fwd, short_conv_fused,
   short_conv_update                       -- the [B,T,D] operators of causal-conv1d-mps
                                              (causal_conv1d_mps/__init__.py:81-419)
+  linear_attention_fn, linear_attention_bwd,
+  linear_attention_update                 -- linear attention with a decay for each head: prompts and
+                                             training, its backward, single tokens
+  copy_pages, reorder_pages, compact_pages,
+  free_pages, PageTable                   -- pages (rows) of a cache of states, moved in place in one launch
   launch_count, last_kernel               -- proof that the CUDA kernels ran
 
 The operators call hand-written CUDA kernels through the C ABI of include/vc1d.h
@@ -17,6 +22,8 @@ that library raises ImportError: there is no CPU or PyTorch fallback.
 from ._cabi import last_kernel, launch_count, library_path, set_pdl, tma_timeouts
 from .ops import (UpdateTable, causal_conv1d_bwd, causal_conv1d_fn, causal_conv1d_fn_multi, causal_conv1d_update,
                   causal_conv1d_update_bwd, causal_conv1d_update_multi, reuse_tile_classes, seq_idx_from_lengths)
+from .linear_attention import linear_attention_bwd, linear_attention_fn, linear_attention_update
+from .cache_pages import PageTable, compact_pages, copy_pages, free_pages, reorder_pages
 from .short_conv import causal_conv1d_fwd, short_conv_fused, short_conv_update
 from . import canon_cache  # noqa: F401  (Canon states on a generation cache: accessors, beam reorder, device transfer)
 from . import compile_ops  # noqa: F401  (registers torch.ops.vc1d.* for torch.compile)
@@ -33,6 +40,14 @@ __all__ = [
     "causal_conv1d_fwd",
     "short_conv_fused",
     "short_conv_update",
+    "linear_attention_fn",
+    "linear_attention_bwd",
+    "linear_attention_update",
+    "PageTable",
+    "copy_pages",
+    "reorder_pages",
+    "compact_pages",
+    "free_pages",
     "launch_count",
     "last_kernel",
     "library_path",

@@ -23,6 +23,10 @@ VC1D_E_NULL, VC1D_E_DTYPE, VC1D_E_WIDTH, VC1D_E_SHAPE = -1, -2, -3, -4
 VC1D_E_STRIDE, VC1D_E_STRUCT, VC1D_E_ACTIVATION, VC1D_E_ALIAS, VC1D_E_TOO_LARGE = -5, -6, -7, -8, -9
 
 KERNEL_AUTO, KERNEL_CHANNEL_LAST, KERNEL_TIME_MAJOR, KERNEL_GENERIC, KERNEL_TMA = 0, 1, 2, 3, 4
+LINEAR_KERNEL_BY_NAME = {None: 0, "auto": 0, "simt": 1, "mma": 2}
+LINEAR_MAX_DIM = 256  # VC1D_LINEAR_MAX_DIM
+PAGES_MAX_TENSORS, PAGES_MAX_PAGES = 128, 8192  # VC1D_PAGES_MAX_TENSORS, VC1D_PAGES_MAX_PAGES
+PAGES_REORDER, PAGES_COPY, PAGES_FREE, PAGES_COMPACT = 0, 1, 2, 3
 KERNEL_BY_NAME = {
     None: KERNEL_AUTO,
     "auto": KERNEL_AUTO,
@@ -217,6 +221,125 @@ class UpdateBwdArgs(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    """struct vc1d_linear_args"""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("seqlen", C.c_int32),
+        ("heads", C.c_int32),
+        ("heads_k", C.c_int32),
+        ("heads_v", C.c_int32),
+        ("dim_k", C.c_int32),
+        ("dim_v", C.c_int32),
+        ("kernel", C.c_int32),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_strides", C.c_int64 * 4),
+        ("k_strides", C.c_int64 * 4),
+        ("v_strides", C.c_int64 * 4),
+        ("out_strides", C.c_int64 * 4),
+        ("log_decay", C.c_void_p),
+        ("mask", C.c_void_p),
+        ("mask_strides", C.c_int64 * 2),
+        ("seq_idx", C.c_void_p),
+        ("seq_strides", C.c_int64 * 2),
+        ("initial_state", C.c_void_p),
+        ("final_state", C.c_void_p),
+        ("initial_strides", C.c_int64 * 4),
+        ("final_strides", C.c_int64 * 4),
+        ("mask_dtype", C.c_int32),
+        ("scale", C.c_float),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+        ("segments", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class LinearBwdArgs(C.Structure):
+    """struct vc1d_linear_bwd_args"""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("segments", C.c_int32),
+        ("f", LinearArgs),
+        ("dout", C.c_void_p),
+        ("dfinal", C.c_void_p),
+        ("dq", C.c_void_p),
+        ("dk", C.c_void_p),
+        ("dv", C.c_void_p),
+        ("dinitial", C.c_void_p),
+        ("dout_strides", C.c_int64 * 4),
+        ("dfinal_strides", C.c_int64 * 4),
+        ("dq_strides", C.c_int64 * 4),
+        ("dk_strides", C.c_int64 * 4),
+        ("dv_strides", C.c_int64 * 4),
+        ("dinitial_strides", C.c_int64 * 4),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+class LinearUpdateArgs(C.Structure):
+    """struct vc1d_linear_update_args"""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("heads", C.c_int32),
+        ("heads_k", C.c_int32),
+        ("heads_v", C.c_int32),
+        ("dim_k", C.c_int32),
+        ("dim_v", C.c_int32),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("out", C.c_void_p),
+        ("state", C.c_void_p),
+        ("log_decay", C.c_void_p),
+        ("mask", C.c_void_p),
+        ("q_strides", C.c_int64 * 3),
+        ("k_strides", C.c_int64 * 3),
+        ("v_strides", C.c_int64 * 3),
+        ("out_strides", C.c_int64 * 3),
+        ("state_strides", C.c_int64 * 4),
+        ("mask_stride", C.c_int64),
+        ("mask_dtype", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class PageTensor(C.Structure):
+    """struct vc1d_page_tensor"""
+
+    _fields_ = [("base", C.c_void_p), ("page_bytes", C.c_int64), ("stride_bytes", C.c_int64)]
+
+
+class PagesArgs(C.Structure):
+    """struct vc1d_pages_args"""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("op", C.c_int32),
+        ("pages", C.c_int32),
+        ("n_tensors", C.c_int32),
+        ("tensors", C.POINTER(PageTensor)),
+        ("source", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("live", C.c_void_p),
+        ("new_index", C.c_void_p),
+        ("count", C.c_void_p),
+        ("n", C.c_int32),
+        ("index_dtype", C.c_int32),
+    ]
+
+
 # every symbol include/vc1d.h declares: name -> (restype, argtypes)
 EXPORTS = {
     "vc1d_prefill": (C.c_int, [C.POINTER(PrefillArgs), C.c_void_p]),
@@ -227,6 +350,16 @@ EXPORTS = {
     "vc1d_update_multi": (C.c_int, [C.POINTER(UpdateArgs), C.c_int32, C.c_void_p]),
     "vc1d_update_bwd": (C.c_int, [C.POINTER(UpdateBwdArgs), C.c_void_p]),
     "vc1d_sizeof_update_bwd_args": (C.c_uint32, []),
+    "vc1d_linear": (C.c_int, [C.POINTER(LinearArgs), C.c_void_p]),
+    "vc1d_linear_workspace": (C.c_int64, [C.POINTER(LinearArgs)]),
+    "vc1d_sizeof_linear_args": (C.c_uint32, []),
+    "vc1d_linear_bwd": (C.c_int, [C.POINTER(LinearBwdArgs), C.c_void_p]),
+    "vc1d_linear_bwd_workspace": (C.c_int64, [C.POINTER(LinearBwdArgs)]),
+    "vc1d_sizeof_linear_bwd_args": (C.c_uint32, []),
+    "vc1d_linear_update": (C.c_int, [C.POINTER(LinearUpdateArgs), C.c_void_p]),
+    "vc1d_sizeof_linear_update_args": (C.c_uint32, []),
+    "vc1d_pages": (C.c_int, [C.POINTER(PagesArgs), C.c_void_p]),
+    "vc1d_sizeof_pages_args": (C.c_uint32, []),
     "vc1d_abi_version": (C.c_int, []),
     "vc1d_sizeof_prefill_args": (C.c_uint32, []),
     "vc1d_sizeof_update_args": (C.c_uint32, []),
@@ -269,6 +402,10 @@ def _load() -> C.CDLL:
         or lib.vc1d_sizeof_update_args() != C.sizeof(UpdateArgs)
         or lib.vc1d_sizeof_prefill_bwd_args() != C.sizeof(PrefillBwdArgs)
         or lib.vc1d_sizeof_update_bwd_args() != C.sizeof(UpdateBwdArgs)
+        or lib.vc1d_sizeof_linear_args() != C.sizeof(LinearArgs)
+        or lib.vc1d_sizeof_linear_bwd_args() != C.sizeof(LinearBwdArgs)
+        or lib.vc1d_sizeof_linear_update_args() != C.sizeof(LinearUpdateArgs)
+        or lib.vc1d_sizeof_pages_args() != C.sizeof(PagesArgs)
     ):
         raise ImportError(f"{path}: argument struct layout differs from the binding; rebuild it")
     return lib

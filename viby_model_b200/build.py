@@ -36,6 +36,10 @@ SOURCES = [
     "prefill_bwd_tma_f16.cu",
     "update.cu",
     "update_bwd.cu",
+    "linear_attention.cu",
+    "linear_attention_simt.cu",
+    "linear_attention_update.cu",
+    "cache_pages.cu",
 ]
 
 NVCC_FLAGS = [

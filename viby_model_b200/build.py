@@ -38,6 +38,8 @@ SOURCES = [
     "update_bwd.cu",
     "linear_attention.cu",
     "linear_attention_simt.cu",
+    "linear_attention_mma_bf16.cu",
+    "linear_attention_mma_f16.cu",
     "linear_attention_update.cu",
     "cache_pages.cu",
 ]

@@ -168,14 +168,36 @@ long long split_bytes(const Launch& l, int segments) {
     return n;
 }
 
-int plan_launch(const Launch& l, int wanted) {
+bool vector_rows(const Rows& r, int eb) {
+    const int per = 16 / eb;
+    return r.sd == 1 && r.sb % per == 0 && r.st % per == 0 && r.sh % per == 0 && (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0;
+}
+bool mma_fits(const Launch& l, int dtype) {
+    if (dtype == VC1D_F32) return false;
+    for (int i = 0; i < l.runs; ++i) {
+        const Run& r = l.run[i];
+        if (r.da % 8 != 0 || r.dv % 8 != 0 || !vector_rows(r.a, 2) || !vector_rows(r.k, 2) || !vector_rows(r.v, 2)) return false;
+    }
+    return true;
+}
+bool use_mma(const Launch& l, int dtype, int kernel) { return kernel != VC1D_LINEAR_SIMT && mma_fits(l, dtype); }
+
+int plan_launch(const Launch& l, int dtype, int kernel, int wanted) {
+    const int slab = slab_of(l, use_mma(l, dtype, kernel));
     long long ctas = 0;
-    for (int i = 0; i < l.runs; ++i) ctas += (long long)l.c.batch * l.c.heads * ((l.run[i].dv + 63) / 64);
+    for (int i = 0; i < l.runs; ++i) ctas += (long long)l.c.batch * l.c.heads * ((l.run[i].dv + slab - 1) / slab);
     return plan_segments(ctas, l.c.seqlen, wanted);
+}
+
+cudaError_t launch_one(const Launch& l, int dtype, bool mma, bool states_only, cudaStream_t s) {
+    if (!mma) return launch_linear_simt(l, dtype, states_only, s);
+    return dtype == VC1D_BF16 ? launch_linear_mma_bf16(l, states_only, s) : launch_linear_mma_f16(l, states_only, s);
 }
 
 // Enqueues the runs of `l`, split along time if the workspace allows it.
 cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, long long ws_bytes, cudaStream_t s) {
+    const bool mma = use_mma(l, dtype, kernel);
+    for (int i = 0; i < l.runs; ++i) l.run[i].out_vec = !l.run[i].out_f32 && vector_rows(l.run[i].o, elem_bytes(dtype));
     if (segments > 1 && (ws == nullptr || ws_bytes < split_bytes(l, segments))) segments = 1;
     const int chunks = (l.c.seqlen + kChunk - 1) / kChunk;
     l.c.segments = segments;
@@ -188,7 +210,7 @@ cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, lo
             l.c.seg_factor[i] = reinterpret_cast<float2*>(ws);
             ws += align16(8LL * (segments - 1) * bh);
         }
-        cudaError_t e = launch_linear_simt(l, dtype, true, s);
+        cudaError_t e = launch_one(l, dtype, mma, true, s);
         if (e != cudaSuccess) return e;
         long long most = 0;
         for (int i = 0; i < l.runs; ++i) most = std::max(most, (long long)l.c.batch * l.c.heads * l.run[i].da * l.run[i].dv);
@@ -198,7 +220,7 @@ cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, lo
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }
-    return launch_linear_simt(l, dtype, false, s);
+    return launch_one(l, dtype, mma, false, s);
 }
 
 Launch forward_launch(const vc1d_linear_args& a) {
@@ -333,7 +355,8 @@ VC1D_API int vc1d_linear(const vc1d_linear_args* a, void* stream) {
     if (a->seqlen == 0 && a->final_state == nullptr) return VC1D_OK;
     if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return VC1D_E_STRIDE;
     lin::Launch l = lin::forward_launch(*a);
-    return (int)lin::enqueue(l, a->dtype, a->kernel, lin::plan_launch(l, a->segments), static_cast<char*>(a->workspace), a->workspace_bytes,
+    if (a->kernel == VC1D_LINEAR_MMA && a->seqlen > 0 && !lin::mma_fits(l, a->dtype)) return VC1D_E_STRIDE;
+    return (int)lin::enqueue(l, a->dtype, a->kernel, lin::plan_launch(l, a->dtype, a->kernel, a->segments), static_cast<char*>(a->workspace), a->workspace_bytes,
                              static_cast<cudaStream_t>(stream));
 }
 
@@ -343,7 +366,7 @@ VC1D_API int64_t vc1d_linear_workspace(const vc1d_linear_args* a) {
     if (st != VC1D_OK) return st;
     if (a->batch == 0 || a->seqlen == 0) return 0;
     const lin::Launch l = lin::forward_launch(*a);
-    return lin::split_bytes(l, lin::plan_launch(l, a->segments));
+    return lin::split_bytes(l, lin::plan_launch(l, a->dtype, a->kernel, a->segments));
 }
 
 VC1D_API int vc1d_linear_bwd(const vc1d_linear_bwd_args* a, void* stream) {
@@ -362,10 +385,11 @@ VC1D_API int vc1d_linear_bwd(const vc1d_linear_bwd_args* a, void* stream) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     lin::Launch fwd, rev;
     lin::backward_launches(*a, &fwd, &rev, part_k, part_v);
+    if (f.kernel == VC1D_LINEAR_MMA && f.seqlen > 0 && !(lin::mma_fits(fwd, f.dtype) && lin::mma_fits(rev, f.dtype))) return VC1D_E_STRIDE;
     cudaError_t e = cudaSuccess;
     // the two launches follow each other on the stream, so they use the same workspace
-    if (f.seqlen > 0) e = lin::enqueue(fwd, f.dtype, f.kernel, lin::plan_launch(fwd, a->segments), split, left, s);
-    if (e == cudaSuccess) e = lin::enqueue(rev, f.dtype, f.kernel, lin::plan_launch(rev, a->segments), split, left, s);
+    if (f.seqlen > 0) e = lin::enqueue(fwd, f.dtype, f.kernel, lin::plan_launch(fwd, f.dtype, f.kernel, a->segments), split, left, s);
+    if (e == cudaSuccess) e = lin::enqueue(rev, f.dtype, f.kernel, lin::plan_launch(rev, f.dtype, f.kernel, a->segments), split, left, s);
     if (e == cudaSuccess && bk > 0)
         e = lin::sum_heads(f.dtype, part_k, lin::rows(a->dk, a->dk_strides, f.heads / f.heads_k), f, f.dim_k, s);
     if (e == cudaSuccess && bv > 0)
@@ -385,7 +409,7 @@ VC1D_API int64_t vc1d_linear_bwd_workspace(const vc1d_linear_bwd_args* a) {
     lin::Launch fwd, rev;
     lin::backward_launches(*a, &fwd, &rev, nullptr, nullptr);
     return lin::part_bytes(f, f.heads_k, f.dim_k) + lin::part_bytes(f, f.heads_v, f.dim_v) +
-           std::max(lin::split_bytes(fwd, lin::plan_launch(fwd, a->segments)), lin::split_bytes(rev, lin::plan_launch(rev, a->segments)));
+           std::max(lin::split_bytes(fwd, lin::plan_launch(fwd, f.dtype, f.kernel, a->segments)), lin::split_bytes(rev, lin::plan_launch(rev, f.dtype, f.kernel, a->segments)));
 }
 
 VC1D_API uint32_t vc1d_sizeof_linear_args(void) { return (uint32_t)sizeof(vc1d_linear_args); }

@@ -42,6 +42,7 @@ struct Run {
     State x0, xT;     // state before the first and after the last token; p may be NULL
     int da, dv;       // channels of a and k (rows of the state), channels of v and out (its columns)
     int out_f32;      // out holds fp32 (partial sums of shared heads), else the I/O type
+    int out_vec;      // out takes 16-byte stores (tensor-core kernel)
     int reverse;      // tokens run from the last to the first (the strides of a, k, v, o already say so)
     int shift;        // 1 in the backward direction
     float s_pair, s_carry, s_add;  // factors on the products inside a chunk, on a X, and on what enters the state
@@ -157,10 +158,22 @@ bool writable(const int (&n)[D], const int64_t (&s)[D]) {
     return true;
 }
 
+// Rows of the state that the tensor-core kernel is compiled for, and the columns of its slabs.  160 rows (Viby's heads)
+// have a variant of their own with slabs of 80: half of 160 columns, and two CTAs per SM.
+inline int rows_of(const Launch& l) {
+    int da = 0;
+    for (int i = 0; i < l.runs; ++i) da = l.run[i].da > da ? l.run[i].da : da;
+    return da <= 64 ? 64 : da <= 128 ? 128 : da <= 160 ? 160 : 256;
+}
+inline int slab_of(const Launch& l, bool mma) { return mma && rows_of(l) == 160 ? 80 : 64; }
+
 }  // namespace lin
 
-// Launchers.  Each returns cudaErrorNotSupported, with nothing launched, when a run does not fit its layout.
+// Launchers.
 // states_only: no outputs; part s of the time axis leaves its own state and total factor in the workspace.
 cudaError_t launch_linear_simt(const lin::Launch& l, int dtype, bool states_only, cudaStream_t s);
+// 16-bit types only; a, k, v with channel stride 1, 16-byte aligned rows, dims a multiple of 8 (lin::mma_fits).
+cudaError_t launch_linear_mma_bf16(const lin::Launch& l, bool states_only, cudaStream_t s);
+cudaError_t launch_linear_mma_f16(const lin::Launch& l, bool states_only, cudaStream_t s);
 
 }  // namespace vc1d

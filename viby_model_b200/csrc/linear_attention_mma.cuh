@@ -1,0 +1,613 @@
+// Linear attention on the tensor cores (16-bit types, channel stride 1, 16-byte aligned rows, head dims a multiple of 8).
+//
+// One CTA of four warps owns one (row, head), a slab of BV state columns and a part of the time axis, and walks its
+// chunks of 64 tokens.  The fp32 state stays in registers for the whole walk: warp w holds the 16-row blocks w, w + 4, ...
+// of the slab.  Per chunk, with warp w on 16 of its queries:
+//     P = q k^T and O = q X          one pass over q's fragments; keys later than the warp's queries are skipped
+//     O = decay O + (decay P) v      P goes from accumulators to operands in registers
+//     X = a^n X + (w k)^T v          k^T straight from shared memory, weighted and split in registers
+// k and v of the next chunk are in flight meanwhile (two buffers); a warp's own rows of q are refilled as soon as it has
+// read them, and carry its part of the output out in between.
+//
+// Roundings.  The state that the queries read and the products inside a chunk are rounded to the I/O type, as operands
+// of the second product: each term of an output meets one such rounding, of the size of the output's own.  The state
+// itself is fp32 in every respect: the weighted keys are split into two (no state asked for: about 16 bits of them) or
+// three bf16 parts (24 bits), fp16 ones into two tf32 parts (22 bits, and no trouble with fp16's range), and a chunk's sum is
+// formed from zero and then added to the state, because the tensor cores truncate where an fp32 add rounds: thousands of
+// accumulations onto one long-lived state would all err towards zero.
+// fp16's range: the rounded state and the products are scaled by powers of two (per CTA, per query) around their maximum.
+#pragma once
+
+#include "linear_attention.cuh"
+
+namespace vc1d {
+namespace lin {
+namespace mma {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+
+struct Info {  // of a chunk's tokens, by one warp two chunks ahead
+    int code[kChunk];
+    float carry[kChunk];  // a^{n_i} for tokens of the sequence that the chunk starts in, else 0
+    float add[kChunk];    // weight of the token's key in the state after the chunk
+    unsigned valid[2];
+    int n_all, run_all;
+};
+
+template <int DAP, int BV>
+struct Layout {
+    // rows padded by 16 bytes: 8 consecutive rows start in 8 different 16-byte bank groups, as ldmatrix wants them
+    static constexpr int kStrideA = DAP + 8, kStrideV = BV + 8;
+    // the state's rows of 80 columns go without (two CTAs of the 160 x 80 variant just fit an SM; two-way conflicts)
+    static constexpr int kStrideX = BV == 80 ? BV : BV + 8;
+    static constexpr int kQ = 0;
+    static constexpr int kK = kQ + kChunk * kStrideA;
+    static constexpr int kV = kK + 2 * kChunk * kStrideA;
+    static constexpr int kX = kV + 2 * kChunk * kStrideV;
+    static constexpr int kEnd = kX + DAP * kStrideX;  // 16-bit elements
+    static constexpr int kBytes = 2 * kEnd + 3 * (int)sizeof(Info) + 8 * kPowers + 16;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int DT>
+struct Half;
+template <>
+struct Half<VC1D_BF16> {
+    __device__ __forceinline__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    __device__ __forceinline__ static float lo(uint32_t v) { return __uint_as_float(v << 16); }
+    __device__ __forceinline__ static float hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+};
+template <>
+struct Half<VC1D_F16> {
+    __device__ __forceinline__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    __device__ __forceinline__ static uint32_t pack(float lo, float hi) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    __device__ __forceinline__ static float lo(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xffffu))); }
+    __device__ __forceinline__ static float hi(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
+};
+
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r & 0xffffe000u;
+}
+
+// 2^k that brings x (>= 0) to [2^13, 2^14), and its inverse; 1 for 0, infinities and NaN.  x below 2^least counts as 2^least.
+__device__ __forceinline__ void scale_around(float x, int least, float* up, float* down) {
+    int e = (int)(__float_as_uint(x) >> 23) - 127;
+    if (x == 0.f || e == 128) e = 13;
+    e = max(least, min(113, e));
+    *up = __uint_as_float((unsigned)(127 + 13 - e) << 23);
+    *down = __uint_as_float((unsigned)(127 - 13 + e) << 23);
+}
+
+// DAP: rows of the state, padded; BV: columns of a slab; PARTS: how finely weighted keys are split (bf16).
+template <int DT, int DAP, int BV, int PARTS, bool STATES>
+__global__ void __launch_bounds__(kThreads) k_linear_mma(const __grid_constant__ Launch l) {
+    using E = Elem<DT>;
+    using T = typename E::type;
+    using Hf = Half<DT>;
+    using L = Layout<DAP, BV>;
+    constexpr int kBlocks = DAP / 16;                         // 16-row blocks of the state
+    constexpr int kMine = (kBlocks + kWarps - 1) / kWarps;    // at most so many of them per warp
+    constexpr int kN = BV / 8;                                // 8-column tiles of a slab
+    constexpr int kUnitsA = DAP / 8, kUnitsV = BV / 8;        // 16-byte units of a row
+    constexpr bool kF16 = DT == VC1D_F16;
+
+    extern __shared__ __align__(16) unsigned char raw[];
+    T* sm = reinterpret_cast<T*>(raw);
+    Info* infos = reinterpret_cast<Info*>(raw + 2 * L::kEnd);
+    float* pw_hi = reinterpret_cast<float*>(raw + 2 * L::kEnd + 3 * sizeof(Info));
+    float* pw_lo = pw_hi + kPowers;
+    float* warp_max = pw_lo + kPowers;  // [kWarps]
+
+    const Run& r = l.run[blockIdx.z];
+    const Common& c = l.c;
+    const int slabs = (r.dv + BV - 1) / BV;
+    const int slab = blockIdx.x % slabs, bh = blockIdx.x / slabs, seg = blockIdx.y;
+    if (bh >= c.batch * c.heads) return;  // a run with fewer slabs than the launch's widest
+    const int b = bh / c.heads, h = bh % c.heads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t4 = lane & 3;
+    const int c0 = slab * BV, cols = min(BV, r.dv - c0);
+    // The later a warp's queries are, the more keys they see.  Every other wave of CTAs deals the 16-row groups out in
+    // reverse, so that the two CTAs of an SM load its four schedulers alike.
+    const int grp = ((blockIdx.x / 148) & 1) ? kWarps - 1 - warp : warp;
+
+    for (int n = tid; n < kPowers; n += kThreads) {
+        const float d = c.log_decay[h];
+        const double x = n == 0 ? 1.0 : exp((double)d * (double)n);
+        const float hi = (float)x;
+        const double lo = x - (double)hi;
+        pw_hi[n] = hi;
+        pw_lo[n] = (isfinite(hi) && lo == lo) ? (float)lo : 0.f;
+    }
+    for (int i = tid; i < L::kEnd / 8; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+
+    const int t_begin = seg * c.seg_chunks * kChunk;
+    const int t_end = min(c.seqlen, t_begin + c.seg_chunks * kChunk);
+    const int chunks = (t_end - t_begin + kChunk - 1) / kChunk;
+    const T* pa = static_cast<const T*>(r.a.p) + (long long)b * r.a.sb + (long long)(h / r.a.group) * r.a.sh;
+    const T* pk = static_cast<const T*>(r.k.p) + (long long)b * r.k.sb + (long long)(h / r.k.group) * r.k.sh;
+    const T* pv = static_cast<const T*>(r.v.p) + (long long)b * r.v.sb + (long long)(h / r.v.group) * r.v.sh + c0;
+    const int ua = r.da / 8, uv = cols / 8;  // units that hold data
+
+    // ---- the state, in registers ----
+    float X[kMine][kN][4];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int blk = warp + kWarps * i;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = blk * 16 + g + (e >> 1) * 8, col = n * 8 + 2 * t4 + (e & 1);
+                float x = 0.f;
+                if (!STATES && blk < kBlocks && row < r.da && col < cols) {
+                    if (seg > 0)
+                        x = c.seg_state[blockIdx.z][((long long)(seg - 1) * c.batch * c.heads + bh) * ((long long)r.da * r.dv) +
+                                                    (long long)row * r.dv + c0 + col];
+                    else if (r.x0.p != nullptr)
+                        x = r.x0.p[(long long)b * r.x0.sb + (long long)h * r.x0.sh + (long long)row * r.x0.sr + (long long)(c0 + col) * r.x0.sc];
+                }
+                X[i][n][e] = x;
+            }
+    }
+    __syncthreads();  // shared memory is zero, the powers are there
+
+    auto fill_info = [&](int chunk) {  // by one warp
+        Info* f = infos + chunk % 3;
+        const int t0 = t_begin + chunk * kChunk;
+        unsigned ok[2], start[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int t = t0 + 32 * half + lane;
+            const long long at = r.reverse ? c.seqlen - 1 - t : t;
+            bool v = t < t_end, s = false;
+            if (v && c.mask != nullptr) v = mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + at * c.mask_st);
+            if (t < t_end && c.seq_idx != nullptr && t > 0) {
+                const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + at * c.seq_st;
+                s = p[0] != (r.reverse ? p[c.seq_st] : p[-c.seq_st]);
+            }
+            ok[half] = __ballot_sync(0xffffffffu, v);
+            start[half] = __ballot_sync(0xffffffffu, s);
+        }
+        const unsigned upto = 0xffffffffu >> (31 - lane);
+        const int n0 = __popc(ok[0]), r0 = __popc(start[0]);
+        const int n_all = n0 + __popc(ok[1]), run_all = r0 + __popc(start[1]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int n = (half ? n0 : 0) + __popc(ok[half] & upto), run = (half ? r0 : 0) + __popc(start[half] & upto);
+            f->code[32 * half + lane] = n + (run << 16);
+            f->carry[32 * half + lane] = run == 0 ? pw_hi[max(n - r.shift, 0)] * r.s_carry : 0.f;
+            f->add[32 * half + lane] = run == run_all ? pw_hi[n_all - n + r.shift] * r.s_add : 0.f;
+        }
+        if (lane == 0) {
+            f->valid[0] = ok[0];
+            f->valid[1] = ok[1];
+            f->n_all = n_all;
+            f->run_all = run_all;
+        }
+    };
+    auto load_kv = [&](int chunk) {
+        const Info* f = infos + chunk % 3;
+        const int t0 = t_begin + chunk * kChunk, buf = chunk & 1;
+        const uint32_t dk = smem_u32(sm + L::kK + buf * kChunk * L::kStrideA), dv = smem_u32(sm + L::kV + buf * kChunk * L::kStrideV);
+        for (int i = tid; i < kChunk * kUnitsA; i += kThreads) {
+            const int row = i / kUnitsA, u = i % kUnitsA;
+            if (u < ua) {
+                const bool ok = f->valid[row >> 5] >> (row & 31) & 1u;
+                cp16(dk + 2 * (row * L::kStrideA + u * 8), ok ? pk + (long long)(t0 + row) * r.k.st + u * 8 : pk, ok);
+            }
+        }
+        for (int i = tid; i < kChunk * kUnitsV; i += kThreads) {
+            const int row = i / kUnitsV, u = i % kUnitsV;
+            if (u < uv) {
+                const bool ok = f->valid[row >> 5] >> (row & 31) & 1u;
+                cp16(dv + 2 * (row * L::kStrideV + u * 8), ok ? pv + (long long)(t0 + row) * r.v.st + u * 8 : pv, ok);
+            }
+        }
+    };
+    T* sq = sm + L::kQ + grp * 16 * L::kStrideA;  // this warp's rows of q
+    auto load_q = [&](int chunk) {
+        const Info* f = infos + chunk % 3;
+        const int t0 = t_begin + chunk * kChunk + grp * 16;
+        const uint32_t d = smem_u32(sq);
+        for (int i = lane; i < 16 * kUnitsA; i += 32) {
+            const int row = i / kUnitsA, u = i % kUnitsA, at = grp * 16 + row;
+            // units past the head's end are cleared too: the output passes through these rows
+            const bool ok = u < ua && (f->valid[at >> 5] >> (at & 31) & 1u);
+            cp16(d + 2 * (row * L::kStrideA + u * 8), ok ? pa + (long long)(t0 + row) * r.a.st + u * 8 : pa, ok);
+        }
+    };
+    float x_down = 1.f;  // fp16: what the rounded state has to be multiplied by
+    auto store_x = [&]() {
+        float up = 1.f;
+        if constexpr (kF16) {
+            float m = warp_max[0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) m = fmaxf(m, warp_max[w]);
+            scale_around(m, -100, &up, &x_down);
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int blk = warp + kWarps * i;
+            if (blk < kBlocks) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    uint32_t* p = reinterpret_cast<uint32_t*>(sm + L::kX + (blk * 16 + g) * L::kStrideX + n * 8 + 2 * t4);
+                    p[0] = Hf::pack(X[i][n][0] * up, X[i][n][1] * up);
+                    p[4 * L::kStrideX] = Hf::pack(X[i][n][2] * up, X[i][n][3] * up);
+                }
+            }
+        }
+    };
+    auto note_max = [&]() {  // fp16: the largest magnitude of the state, per warp
+        if constexpr (kF16) {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(X[i][n][e]));
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            if (lane == 0) warp_max[warp] = m;
+        }
+    };
+
+    if (chunks > 0) {
+        if (warp == 0) fill_info(0);
+        if (warp == 1 && chunks > 1) fill_info(1);
+        if (!STATES) note_max();
+        __syncthreads();
+        load_kv(0);
+        if (!STATES) {
+            load_q(0);
+            store_x();
+        }
+        cp_commit();
+    }
+    double seg_factor = 1.0;
+
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        cp_wait();
+        __syncthreads();  // this chunk's tokens and the rounded state are there; the other buffers are free
+        const Info& f = infos[chunk % 3];
+        if (chunk + 1 < chunks) load_kv(chunk + 1);
+        cp_commit();
+        if (chunk + 2 < chunks && warp == (chunk & 3)) fill_info(chunk + 2);
+        const T* sk = sm + L::kK + (chunk & 1) * kChunk * L::kStrideA;
+        const T* sv = sm + L::kV + (chunk & 1) * kChunk * L::kStrideV;
+
+        if (!STATES) {
+            // ---- P = q k^T, O = q X ----
+            float P[8][4], O[kN][4];
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) P[n][e] = 0.f;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) O[n][e] = 0.f;
+            const uint32_t aq = smem_u32(sq + (lane & 15) * L::kStrideA + (lane >> 4) * 8);
+            const uint32_t bk = smem_u32(sk + ((lane & 7) + (lane >> 4) * 8) * L::kStrideA + (lane >> 3 & 1) * 8);
+            const uint32_t bx = smem_u32(sm + L::kX + ((lane & 7) + (lane >> 3 & 1) * 8) * L::kStrideX + (lane >> 4) * 8);
+#pragma unroll 2
+            for (int kk = 0; kk < kBlocks; ++kk) {
+                uint32_t a[4];
+                ldsm4(a, aq + 2 * (kk * 16));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j <= grp) {
+                        uint32_t kb[4];
+                        ldsm4(kb, bk + 2 * (j * 16 * L::kStrideA + kk * 16));
+                        Hf::mma(P[2 * j], a, kb[0], kb[1]);
+                        Hf::mma(P[2 * j + 1], a, kb[2], kb[3]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kN; n += 2) {
+                    uint32_t xb[4];
+                    ldsm4t(xb, bx + 2 * (kk * 16 * L::kStrideX + n * 8));
+                    Hf::mma(O[n], a, xb[0], xb[1]);
+                    Hf::mma(O[n + 1], a, xb[2], xb[3]);
+                }
+            }
+            // ---- decays ----
+            const int i0 = grp * 16 + g;
+            const int code0 = f.code[i0], code1 = f.code[i0 + 8];
+            float f0 = f.carry[i0] * x_down, f1 = f.carry[i0 + 8] * x_down;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                if (n <= 2 * grp + 1) {
+                    const int2 cj = *reinterpret_cast<const int2*>(f.code + n * 8 + 2 * t4);
+                    const unsigned l00 = (unsigned)(code0 - cj.x), l01 = (unsigned)(code0 - cj.y);
+                    const unsigned l10 = (unsigned)(code1 - cj.x), l11 = (unsigned)(code1 - cj.y);
+                    P[n][0] = l00 <= kChunk ? P[n][0] * (pw_hi[l00] * r.s_pair) : 0.f;
+                    P[n][1] = l01 <= kChunk ? P[n][1] * (pw_hi[l01] * r.s_pair) : 0.f;
+                    P[n][2] = l10 <= kChunk ? P[n][2] * (pw_hi[l10] * r.s_pair) : 0.f;
+                    P[n][3] = l11 <= kChunk ? P[n][3] * (pw_hi[l11] * r.s_pair) : 0.f;
+                }
+            }
+            float down0 = 1.f, down1 = 1.f;
+            if constexpr (kF16) {
+                float m0 = 0.f, m1 = 0.f, up0, up1;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    m0 = fmaxf(m0, fmaxf(fabsf(P[n][0]), fabsf(P[n][1])));
+                    m1 = fmaxf(m1, fmaxf(fabsf(P[n][2]), fabsf(P[n][3])));
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
+                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
+                }
+                // products below 2^-20 reach fp16 outputs as less than its smallest step, so they need no larger factor,
+                // which what the state adds to this accumulator would have to bear too
+                scale_around(m0, -20, &up0, &down0);
+                scale_around(m1, -20, &up1, &down1);
+                f0 *= up0;
+                f1 *= up1;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    P[n][0] *= up0, P[n][1] *= up0;
+                    P[n][2] *= up1, P[n][3] *= up1;
+                }
+            }
+            const bool in0 = (code0 >> 16) == 0, in1 = (code1 >> 16) == 0;  // a later sequence takes nothing of X, infinities neither
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                O[n][0] = in0 ? O[n][0] * f0 : 0.f, O[n][1] = in0 ? O[n][1] * f0 : 0.f;
+                O[n][2] = in1 ? O[n][2] * f1 : 0.f, O[n][3] = in1 ? O[n][3] * f1 : 0.f;
+            }
+            // ---- O += P v ----
+            const uint32_t bv = smem_u32(sv + ((lane & 7) + (lane >> 3 & 1) * 8) * L::kStrideV + (lane >> 4) * 8);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                if (kk <= grp) {
+                    const uint32_t a[4] = {Hf::pack(P[2 * kk][0], P[2 * kk][1]), Hf::pack(P[2 * kk][2], P[2 * kk][3]),
+                                           Hf::pack(P[2 * kk + 1][0], P[2 * kk + 1][1]), Hf::pack(P[2 * kk + 1][2], P[2 * kk + 1][3])};
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        uint32_t vb[4];
+                        ldsm4t(vb, bv + 2 * (kk * 16 * L::kStrideV + n * 8));
+                        Hf::mma(O[n], a, vb[0], vb[1]);
+                        Hf::mma(O[n + 1], a, vb[2], vb[3]);
+                    }
+                }
+            }
+            // ---- out ----
+            const bool ok0 = f.valid[i0 >> 5] >> (i0 & 31) & 1u, ok1 = f.valid[(i0 + 8) >> 5] >> ((i0 + 8) & 31) & 1u;
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                O[n][0] = ok0 ? O[n][0] * down0 : 0.f, O[n][1] = ok0 ? O[n][1] * down0 : 0.f;
+                O[n][2] = ok1 ? O[n][2] * down1 : 0.f, O[n][3] = ok1 ? O[n][3] * down1 : 0.f;
+            }
+            const int t0 = t_begin + chunk * kChunk + grp * 16;
+            const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
+            if (r.out_vec) {
+                __syncwarp();  // every lane has read its fragments of q
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    uint32_t* p = reinterpret_cast<uint32_t*>(sq + g * L::kStrideA + n * 8 + 2 * t4);
+                    p[0] = Hf::pack(O[n][0], O[n][1]);
+                    p[4 * L::kStrideA] = Hf::pack(O[n][2], O[n][3]);
+                }
+                __syncwarp();
+                T* po = const_cast<T*>(static_cast<const T*>(r.o.p)) + obase + c0;
+#pragma unroll
+                for (int i = lane; i < 16 * kUnitsV; i += 32) {
+                    const int row = i / kUnitsV, u = i % kUnitsV;
+                    if (u < uv && t0 + row < t_end)
+                        st_vec(po + (long long)(t0 + row) * r.o.st + u * 8, *reinterpret_cast<const uint4*>(sq + row * L::kStrideA + u * 8));
+                }
+                __syncwarp();
+            } else {
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int t = t0 + g + (e >> 1) * 8, col = n * 8 + 2 * t4 + (e & 1);
+                        if (t < t_end && col < cols) {
+                            const float o = O[n][e];
+                            const long long at = obase + (long long)t * r.o.st + (long long)(c0 + col) * r.o.sd;
+                            if (r.out_f32)
+                                const_cast<float*>(static_cast<const float*>(r.o.p))[at] = o;
+                            else
+                                const_cast<T*>(static_cast<const T*>(r.o.p))[at] = E::from_float(o);
+                        }
+                    }
+                __syncwarp();
+            }
+            if (chunk + 1 < chunks) load_q(chunk + 1);
+            cp_commit();
+        }
+
+        // ---- X = a^n X + (w k)^T v ----
+        const bool last_state = STATES || chunk + 1 < chunks || seg < c.segments - 1 || r.xT.p != nullptr;
+        if (last_state) {
+            const float2 f = make_float2(pw_hi[infos[chunk % 3].n_all], pw_lo[infos[chunk % 3].n_all]);
+            const bool keep = infos[chunk % 3].run_all == 0;
+            if (STATES) seg_factor = keep ? seg_factor * ((double)f.x + (double)f.y) : 0.0;
+            const float* add = infos[chunk % 3].add;
+            const uint32_t ak = smem_u32(sk + ((lane & 7) + (lane >> 4) * 8) * L::kStrideA + (lane >> 3 & 1) * 8);
+            // two k-steps of one column tile per load: keys 0-31 (or 32-63) of 8 columns
+            const uint32_t bv = smem_u32(sv + lane * L::kStrideV);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const int blk = warp + kWarps * i;
+                if (blk >= kBlocks) continue;
+                // the weighted keys of this block of rows, split
+                constexpr int kRegs = kF16 ? 16 : 4 * PARTS;
+                uint32_t A[4][kRegs];
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    uint32_t kf[4];
+                    ldsm4t(kf, ak + 2 * (kk * 16 * L::kStrideA + blk * 16));
+                    const float2 w0 = *reinterpret_cast<const float2*>(add + kk * 16 + 2 * t4);
+                    const float2 w1 = *reinterpret_cast<const float2*>(add + kk * 16 + 8 + 2 * t4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 w = e < 2 ? w0 : w1;
+                        float x = Hf::lo(kf[e]) * w.x, y = Hf::hi(kf[e]) * w.y;
+                        if constexpr (kF16) {
+                            // [step e/2][part][operand register]: keys 2t go to the first, 2t + 1 to the second half of a k-step
+                            const int at = (e >> 1) * 8 + (e & 1);
+                            A[kk][at] = to_tf32(x);
+                            A[kk][at + 2] = to_tf32(y);
+                            A[kk][at + 4] = to_tf32(x - __uint_as_float(A[kk][at]));
+                            A[kk][at + 6] = to_tf32(y - __uint_as_float(A[kk][at + 2]));
+                        } else {
+#pragma unroll
+                            for (int p = 0; p < PARTS; ++p) {
+                                const uint32_t v = Hf::pack(x, y);
+                                A[kk][4 * p + e] = v;
+                                if (p + 1 < PARTS) {
+                                    x -= Hf::lo(v);
+                                    y -= Hf::hi(v);
+                                }
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kN; n += 2) {
+                    float acc[2][4] = {};
+                    uint32_t vb[2][2][4];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        ldsm4t(vb[j][0], bv + 2 * ((n + j) * 8));
+                        ldsm4t(vb[j][1], bv + 2 * (32 * L::kStrideV + (n + j) * 8));
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t b0 = vb[j][kk >> 1][2 * (kk & 1)], b1 = vb[j][kk >> 1][2 * (kk & 1) + 1];
+                            if constexpr (kF16) {
+                                const uint32_t p0 = __float_as_uint(Hf::lo(b0)), p1 = __float_as_uint(Hf::hi(b0));
+                                const uint32_t q0 = __float_as_uint(Hf::lo(b1)), q1 = __float_as_uint(Hf::hi(b1));
+                                mma_tf32(acc[j], A[kk][4], A[kk][5], A[kk][6], A[kk][7], p0, p1);
+                                mma_tf32(acc[j], A[kk][12], A[kk][13], A[kk][14], A[kk][15], q0, q1);
+                                mma_tf32(acc[j], A[kk][0], A[kk][1], A[kk][2], A[kk][3], p0, p1);
+                                mma_tf32(acc[j], A[kk][8], A[kk][9], A[kk][10], A[kk][11], q0, q1);
+                            } else {
+#pragma unroll
+                                for (int p = PARTS - 1; p >= 0; --p) {
+                                    const uint32_t a[4] = {A[kk][4 * p], A[kk][4 * p + 1], A[kk][4 * p + 2], A[kk][4 * p + 3]};
+                                    Hf::mma(acc[j], a, b0, b1);
+                                }
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            X[i][n + j][e] = keep ? fmaf(X[i][n + j][e], f.x, fmaf(X[i][n + j][e], f.y, acc[j][e])) : acc[j][e];
+                }
+            }
+        }
+        if (!STATES && chunk + 1 < chunks) {
+            note_max();
+            __syncthreads();  // every warp has read the rounded state
+            store_x();
+        }
+    }
+
+    // ---- the state after the last token ----
+    const bool write_final = !STATES && seg == c.segments - 1 && r.xT.p != nullptr;
+    if (STATES || write_final) {
+        float* dst = STATES ? c.seg_state[blockIdx.z] + ((long long)seg * c.batch * c.heads + bh) * ((long long)r.da * r.dv)
+                            : r.xT.p + (long long)b * r.xT.sb + (long long)h * r.xT.sh;
+        const long long sr = STATES ? r.dv : r.xT.sr, sc = STATES ? 1 : r.xT.sc;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int blk = warp + kWarps * i;
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = blk * 16 + g + (e >> 1) * 8, col = n * 8 + 2 * t4 + (e & 1);
+                    if (blk < kBlocks && row < r.da && col < cols) dst[(long long)row * sr + (long long)(c0 + col) * sc] = X[i][n][e];
+                }
+        }
+        if (STATES && slab == 0 && tid == 0) {
+            const float hi = (float)seg_factor;
+            c.seg_factor[blockIdx.z][(long long)seg * c.batch * c.heads + bh] = make_float2(hi, (float)(seg_factor - (double)hi));
+        }
+    }
+}
+
+template <int DT, int DAP, int BV, int PARTS, bool STATES>
+cudaError_t launch(const Launch& l, cudaStream_t s) {
+    constexpr int smem = Layout<DAP, BV>::kBytes;
+    int slabs = 0;
+    for (int i = 0; i < l.runs; ++i) slabs = max(slabs, (l.run[i].dv + BV - 1) / BV);
+    auto kernel = k_linear_mma<DT, DAP, BV, PARTS, STATES>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)(l.c.batch * l.c.heads * slabs), STATES ? l.c.segments - 1 : l.c.segments, l.runs);
+    note_launch(STATES ? "linear_mma_states" : "linear_mma");
+    kernel<<<grid, kThreads, smem, s>>>(l);
+    return cudaGetLastError();
+}
+
+template <int DT, int DAP, int BV>
+cudaError_t launch_parts(const Launch& l, bool states, cudaStream_t s) {
+    bool exact = states;  // a split launch joins fp32 states
+    for (int i = 0; i < l.runs; ++i) exact = exact || l.run[i].xT.p != nullptr;
+    if (states) return launch<DT, DAP, BV, DT == VC1D_F16 ? 2 : 3, true>(l, s);
+    if (exact && DT != VC1D_F16) return launch<DT, DAP, BV, 3, false>(l, s);
+    return launch<DT, DAP, BV, 2, false>(l, s);
+}
+
+template <int DT>
+cudaError_t launch_type(const Launch& l, bool states, cudaStream_t s) {
+    switch (rows_of(l)) {
+        case 64: return launch_parts<DT, 64, 64>(l, states, s);
+        case 128: return launch_parts<DT, 128, 64>(l, states, s);
+        case 160: return launch_parts<DT, 160, 80>(l, states, s);
+        default: return launch_parts<DT, 256, 64>(l, states, s);
+    }
+}
+
+}  // namespace mma
+}  // namespace lin
+}  // namespace vc1d

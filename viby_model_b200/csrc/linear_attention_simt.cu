@@ -163,15 +163,16 @@ __global__ void __launch_bounds__(kThreads) k_linear_simt(const __grid_constant_
             for (int i = 0; i < 4; ++i) {
                 const int t = t0 + ti + i;
                 if (t >= t_end) continue;
+                const bool ok = info.valid[(ti + i) >> 5] >> ((ti + i) & 31) & 1u;
                 const long long base = (long long)b * r.o.sb + (long long)t * r.o.st + (long long)h * r.o.sh;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (tj + j >= cols) continue;
                     const long long at = base + (long long)(c0 + tj + j) * r.o.sd;
                     if (r.out_f32)
-                        const_cast<float*>(static_cast<const float*>(r.o.p))[at] = out[i][j];
+                        const_cast<float*>(static_cast<const float*>(r.o.p))[at] = ok ? out[i][j] : 0.f;
                     else
-                        const_cast<T*>(static_cast<const T*>(r.o.p))[at] = E::from_float(out[i][j]);
+                        const_cast<T*>(static_cast<const T*>(r.o.p))[at] = E::from_float(ok ? out[i][j] : 0.f);
                 }
             }
         }

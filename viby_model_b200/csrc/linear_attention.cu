@@ -151,9 +151,9 @@ int plan_segments(long long ctas, int seqlen, int wanted) {
     const int chunks = (seqlen + kChunk - 1) / kChunk;
     int n = wanted;
     if (n == 0) {
-        const long long full = 2LL * sm_count();  // two CTAs per SM
+        const long long full = 2LL * sm_count();  // two CTAs per SM; no more than that: one wave
         // a part costs a state's worth of work more (its keys and values are read twice), so it is at least 4 chunks
-        n = ctas >= sm_count() ? 1 : (int)std::min<long long>((full + ctas - 1) / std::max(1LL, ctas), std::max(1, chunks / 4));
+        n = ctas >= sm_count() ? 1 : (int)std::min<long long>(full / std::max(1LL, ctas), std::max(1, chunks / 4));
     }
     n = std::max(1, std::min({n, kMaxSegments, chunks}));
     const int per = (chunks + n - 1) / std::max(n, 1);

@@ -346,7 +346,8 @@ VC1D_API uint32_t vc1d_sizeof_update_bwd_args(void);
 enum {
     VC1D_LINEAR_AUTO = 0,
     VC1D_LINEAR_SIMT = 1,  /* fp32 pipes: any strides, every type */
-    VC1D_LINEAR_MMA = 2    /* tensor cores: 16-bit types, channel stride 1, 16-byte aligned rows */
+    VC1D_LINEAR_MMA = 2,   /* warp-level tensor cores: 16-bit types, channel stride 1, 16-byte aligned rows, dims a multiple of 8 */
+    VC1D_LINEAR_TC = 3     /* tcgen05 tensor cores: bf16, as VC1D_LINEAR_MMA, dims up to 160 */
 };
 
 typedef struct vc1d_linear_args {
@@ -489,7 +490,7 @@ VC1D_API uint64_t vc1d_launch_count(void);
 
 /* Name of the kernel the most recent launcher call on this thread selected ("channel_last",
  * "time_major", "generic", "tma", "update_vec", "update_lane", "update_generic", "bwd_tma", "bwd_generic",
- * "update_bwd", "linear_simt", "linear_mma", "linear_update", "pages").  Per host thread: a backward pass run by an autograd worker thread does not show
+ * "update_bwd", "linear_simt", "linear_mma", "linear_tc", "linear_update", "pages").  Per host thread: a backward pass run by an autograd worker thread does not show
  * up in the thread that called the forward. */
 VC1D_API const char* vc1d_last_kernel(void);
 
@@ -499,7 +500,7 @@ VC1D_API const char* vc1d_last_kernel(void);
    table there can be kept.  Bits 8 and up: the slot (0, 1, 2).  No reference counterpart. */
 VC1D_API int vc1d_last_class_table(void);
 
-/* Number of bounded mbarrier waits that expired inside the TMA-staged kernels since the process
+/* Number of bounded mbarrier waits that expired inside the TMA-staged and tcgen05 kernels since the process
  * started (0 in a healthy run; a CTA whose wait expires abandons its remaining tiles).  Reads a
  * device counter with a synchronising copy: call it after the stream has been synchronised. */
 VC1D_API unsigned int vc1d_tma_timeouts(void);

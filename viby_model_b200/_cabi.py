@@ -23,7 +23,7 @@ VC1D_E_NULL, VC1D_E_DTYPE, VC1D_E_WIDTH, VC1D_E_SHAPE = -1, -2, -3, -4
 VC1D_E_STRIDE, VC1D_E_STRUCT, VC1D_E_ACTIVATION, VC1D_E_ALIAS, VC1D_E_TOO_LARGE = -5, -6, -7, -8, -9
 
 KERNEL_AUTO, KERNEL_CHANNEL_LAST, KERNEL_TIME_MAJOR, KERNEL_GENERIC, KERNEL_TMA = 0, 1, 2, 3, 4
-LINEAR_KERNEL_BY_NAME = {None: 0, "auto": 0, "simt": 1, "mma": 2}
+LINEAR_KERNEL_BY_NAME = {None: 0, "auto": 0, "simt": 1, "mma": 2, "tc": 3}
 LINEAR_MAX_DIM = 256  # VC1D_LINEAR_MAX_DIM
 PAGES_MAX_TENSORS, PAGES_MAX_PAGES = 128, 8192  # VC1D_PAGES_MAX_TENSORS, VC1D_PAGES_MAX_PAGES
 PAGES_REORDER, PAGES_COPY, PAGES_FREE, PAGES_COMPACT = 0, 1, 2, 3

@@ -40,6 +40,7 @@ SOURCES = [
     "linear_attention_simt.cu",
     "linear_attention_mma_bf16.cu",
     "linear_attention_mma_f16.cu",
+    "linear_attention_tc.cu",
     "linear_attention_update.cu",
     "cache_pages.cu",
 ]

@@ -84,7 +84,7 @@ int check(const vc1d_linear_args* a) {
     if (a->batch < 0 || a->seqlen < 0 || a->heads < 1 || a->heads_k < 1 || a->heads_v < 1 || a->dim_k < 1 || a->dim_v < 1)
         return VC1D_E_SHAPE;
     if (a->heads % a->heads_k != 0 || a->heads % a->heads_v != 0) return VC1D_E_SHAPE;
-    if (a->kernel < VC1D_LINEAR_AUTO || a->kernel > VC1D_LINEAR_MMA || a->segments < 0 || a->segments > kMaxSegments) return VC1D_E_SHAPE;
+    if (a->kernel < VC1D_LINEAR_AUTO || a->kernel > VC1D_LINEAR_TC || a->segments < 0 || a->segments > kMaxSegments) return VC1D_E_SHAPE;
     if (a->dim_k > kMaxDim || a->dim_v > kMaxDim || a->seqlen > (1 << 30)) return VC1D_E_TOO_LARGE;
     if ((long long)a->batch * a->heads * (kMaxDim / 16) > 0x7fffffffLL) return VC1D_E_TOO_LARGE;
     if (a->seq_idx != nullptr && (a->mask != nullptr || a->initial_state != nullptr || a->final_state != nullptr)) return VC1D_E_SHAPE;
@@ -146,20 +146,6 @@ Common common_of(const vc1d_linear_args& a) {
 
 constexpr long long align16(long long n) { return (n + 15) & ~15LL; }
 
-// Parts of the time axis of a launch with `ctas` CTAs when it is not split.
-int plan_segments(long long ctas, int seqlen, int wanted) {
-    const int chunks = (seqlen + kChunk - 1) / kChunk;
-    int n = wanted;
-    if (n == 0) {
-        const long long full = 2LL * sm_count();  // two CTAs per SM; no more than that: one wave
-        // a part costs a state's worth of work more (its keys and values are read twice), so it is at least 4 chunks
-        n = ctas >= sm_count() ? 1 : (int)std::min<long long>(full / std::max(1LL, ctas), std::max(1, chunks / 4));
-    }
-    n = std::max(1, std::min({n, kMaxSegments, chunks}));
-    const int per = (chunks + n - 1) / std::max(n, 1);
-    return per > 0 ? std::max(1, (chunks + per - 1) / per) : 1;  // no part is empty
-}
-
 long long split_bytes(const Launch& l, int segments) {
     long long n = 0;
     if (segments > 1)
@@ -180,26 +166,45 @@ bool mma_fits(const Launch& l, int dtype) {
     }
     return true;
 }
-bool use_mma(const Launch& l, int dtype, int kernel) { return kernel != VC1D_LINEAR_SIMT && mma_fits(l, dtype); }
-
-int plan_launch(const Launch& l, int dtype, int kernel, int wanted) {
-    const int slab = slab_of(l, use_mma(l, dtype, kernel));
-    long long ctas = 0;
-    for (int i = 0; i < l.runs; ++i) ctas += (long long)l.c.batch * l.c.heads * ((l.run[i].dv + slab - 1) / slab);
-    return plan_segments(ctas, l.c.seqlen, wanted);
+Kind pick(const Launch& l, int dtype, int kernel) {
+    if (kernel == VC1D_LINEAR_SIMT || !mma_fits(l, dtype)) return kSimt;
+    return kernel != VC1D_LINEAR_MMA && dtype == VC1D_BF16 && largest_rows(l) <= 160 ? kTc : kMma;
 }
 
-cudaError_t launch_one(const Launch& l, int dtype, bool mma, bool states_only, cudaStream_t s) {
-    if (!mma) return launch_linear_simt(l, dtype, states_only, s);
+// whether the kernel that the caller names takes this launch
+bool kernel_fits(const Launch& l, int dtype, int kernel) {
+    return kernel == VC1D_LINEAR_AUTO || kernel == VC1D_LINEAR_SIMT || pick(l, dtype, kernel) == (kernel == VC1D_LINEAR_TC ? kTc : kMma);
+}
+
+// Parts of the time axis.
+int plan_launch(const Launch& l, int dtype, int kernel, int wanted) {
+    const Kind kind = pick(l, dtype, kernel);
+    const int slab = slab_of(l, kind), chunks = (l.c.seqlen + chunk_of(kind) - 1) / chunk_of(kind);
+    long long ctas = 0;
+    for (int i = 0; i < l.runs; ++i) ctas += (long long)l.c.batch * l.c.heads * ((l.run[i].dv + slab - 1) / slab);
+    int n = wanted;
+    if (n == 0) {
+        // no more CTAs than run at once; a part costs its keys and values once more, so it is at least 256 tokens
+        const long long full = (long long)ctas_per_sm(l, kind) * sm_count();
+        n = ctas >= sm_count() ? 1 : (int)std::min<long long>(full / std::max(1LL, ctas), std::max(1, l.c.seqlen / 256));
+    }
+    n = std::max(1, std::min({n, kMaxSegments, chunks}));
+    const int per = (chunks + n - 1) / n;
+    return per > 0 ? std::max(1, (chunks + per - 1) / per) : 1;  // no part is empty
+}
+
+cudaError_t launch_one(const Launch& l, int dtype, Kind kind, bool states_only, cudaStream_t s) {
+    if (kind == kSimt) return launch_linear_simt(l, dtype, states_only, s);
+    if (kind == kTc) return launch_linear_tc(l, states_only, s);
     return dtype == VC1D_BF16 ? launch_linear_mma_bf16(l, states_only, s) : launch_linear_mma_f16(l, states_only, s);
 }
 
 // Enqueues the runs of `l`, split along time if the workspace allows it.
 cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, long long ws_bytes, cudaStream_t s) {
-    const bool mma = use_mma(l, dtype, kernel);
+    const Kind kind = pick(l, dtype, kernel);
     for (int i = 0; i < l.runs; ++i) l.run[i].out_vec = !l.run[i].out_f32 && vector_rows(l.run[i].o, elem_bytes(dtype));
     if (segments > 1 && (ws == nullptr || ws_bytes < split_bytes(l, segments))) segments = 1;
-    const int chunks = (l.c.seqlen + kChunk - 1) / kChunk;
+    const int chunks = (l.c.seqlen + chunk_of(kind) - 1) / chunk_of(kind);
     l.c.segments = segments;
     l.c.seg_chunks = std::max(1, (chunks + segments - 1) / segments);
     if (segments > 1) {
@@ -210,7 +215,7 @@ cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, lo
             l.c.seg_factor[i] = reinterpret_cast<float2*>(ws);
             ws += align16(8LL * (segments - 1) * bh);
         }
-        cudaError_t e = launch_one(l, dtype, mma, true, s);
+        cudaError_t e = launch_one(l, dtype, kind, true, s);
         if (e != cudaSuccess) return e;
         long long most = 0;
         for (int i = 0; i < l.runs; ++i) most = std::max(most, (long long)l.c.batch * l.c.heads * l.run[i].da * l.run[i].dv);
@@ -220,7 +225,7 @@ cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, lo
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }
-    return launch_one(l, dtype, mma, false, s);
+    return launch_one(l, dtype, kind, false, s);
 }
 
 Launch forward_launch(const vc1d_linear_args& a) {
@@ -355,7 +360,7 @@ VC1D_API int vc1d_linear(const vc1d_linear_args* a, void* stream) {
     if (a->seqlen == 0 && a->final_state == nullptr) return VC1D_OK;
     if ((reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0) return VC1D_E_STRIDE;
     lin::Launch l = lin::forward_launch(*a);
-    if (a->kernel == VC1D_LINEAR_MMA && a->seqlen > 0 && !lin::mma_fits(l, a->dtype)) return VC1D_E_STRIDE;
+    if (a->seqlen > 0 && !lin::kernel_fits(l, a->dtype, a->kernel)) return VC1D_E_STRIDE;
     return (int)lin::enqueue(l, a->dtype, a->kernel, lin::plan_launch(l, a->dtype, a->kernel, a->segments), static_cast<char*>(a->workspace), a->workspace_bytes,
                              static_cast<cudaStream_t>(stream));
 }
@@ -385,7 +390,7 @@ VC1D_API int vc1d_linear_bwd(const vc1d_linear_bwd_args* a, void* stream) {
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     lin::Launch fwd, rev;
     lin::backward_launches(*a, &fwd, &rev, part_k, part_v);
-    if (f.kernel == VC1D_LINEAR_MMA && f.seqlen > 0 && !(lin::mma_fits(fwd, f.dtype) && lin::mma_fits(rev, f.dtype))) return VC1D_E_STRIDE;
+    if (f.seqlen > 0 && !(lin::kernel_fits(fwd, f.dtype, f.kernel) && lin::kernel_fits(rev, f.dtype, f.kernel))) return VC1D_E_STRIDE;
     cudaError_t e = cudaSuccess;
     // the two launches follow each other on the stream, so they use the same workspace
     if (f.seqlen > 0) e = lin::enqueue(fwd, f.dtype, f.kernel, lin::plan_launch(fwd, f.dtype, f.kernel, a->segments), split, left, s);

@@ -158,14 +158,23 @@ bool writable(const int (&n)[D], const int64_t (&s)[D]) {
     return true;
 }
 
-// Rows of the state that the tensor-core kernel is compiled for, and the columns of its slabs.  160 rows (Viby's heads)
-// have a variant of their own with slabs of 80: half of 160 columns, and two CTAs per SM.
-inline int rows_of(const Launch& l) {
+// The kernels.  kMma: warp-level products, 16-bit types, any head.  kTc: tcgen05, bf16, heads up to 160.
+enum Kind { kSimt, kMma, kTc };
+
+inline int largest_rows(const Launch& l) {
     int da = 0;
     for (int i = 0; i < l.runs; ++i) da = l.run[i].da > da ? l.run[i].da : da;
+    return da;
+}
+// Rows of the state that kMma is compiled for; columns of a slab; tokens of a chunk; CTAs that share an SM.  160 rows
+// (Viby's heads) have a kMma variant of their own with slabs of 80: half of 160 columns, and two CTAs per SM.
+inline int mma_rows(const Launch& l) {
+    const int da = largest_rows(l);
     return da <= 64 ? 64 : da <= 128 ? 128 : da <= 160 ? 160 : 256;
 }
-inline int slab_of(const Launch& l, bool mma) { return mma && rows_of(l) == 160 ? 80 : 64; }
+inline int slab_of(const Launch& l, Kind k) { return k == kMma && mma_rows(l) == 160 ? 80 : 64; }
+inline int chunk_of(Kind k) { return k == kTc ? 128 : kChunk; }
+inline int ctas_per_sm(const Launch& l, Kind k) { return k == kMma && mma_rows(l) <= 160 ? 2 : 1; }
 
 }  // namespace lin
 
@@ -175,5 +184,7 @@ cudaError_t launch_linear_simt(const lin::Launch& l, int dtype, bool states_only
 // 16-bit types only; a, k, v with channel stride 1, 16-byte aligned rows, dims a multiple of 8 (lin::mma_fits).
 cudaError_t launch_linear_mma_bf16(const lin::Launch& l, bool states_only, cudaStream_t s);
 cudaError_t launch_linear_mma_f16(const lin::Launch& l, bool states_only, cudaStream_t s);
+// bf16, as above and at most 160 state rows in every run.
+cudaError_t launch_linear_tc(const lin::Launch& l, bool states_only, cudaStream_t s);
 
 }  // namespace vc1d

@@ -673,7 +673,7 @@ cudaError_t launch(const Launch& l, cudaStream_t s) {
 
 template <int DT>
 cudaError_t launch_type(const Launch& l, bool states, cudaStream_t s) {
-    switch (rows_of(l)) {
+    switch (mma_rows(l)) {
         case 64: return states ? launch<DT, 64, 64, true>(l, s) : launch<DT, 64, 64, false>(l, s);
         case 128: return states ? launch<DT, 128, 64, true>(l, s) : launch<DT, 128, 64, false>(l, s);
         case 160: return states ? launch<DT, 160, 80, true>(l, s) : launch<DT, 160, 80, false>(l, s);

@@ -166,9 +166,24 @@ bool mma_fits(const Launch& l, int dtype) {
     }
     return true;
 }
+// Tensor maps have no zero strides (broadcast inputs) and none of 2^40 bytes.
+bool tma_fits(const Launch& l) {
+    if (!tma_available()) return false;
+    for (int i = 0; i < l.runs; ++i) {
+        const Run& r = l.run[i];
+        for (const Rows* x : {&r.a, &r.k, &r.v}) {
+            const long long st = x->st < 0 ? -x->st : x->st, most = 1LL << 38;
+            if ((l.c.seqlen > 1 && (st == 0 || st > most)) || (l.c.heads / x->group > 1 && (x->sh <= 0 || x->sh > most)) ||
+                (l.c.batch > 1 && (x->sb <= 0 || x->sb > most)))
+                return false;
+            if ((x->st < 0) != (r.reverse != 0) && l.c.seqlen > 1) return false;
+        }
+    }
+    return true;
+}
 Kind pick(const Launch& l, int dtype, int kernel) {
     if (kernel == VC1D_LINEAR_SIMT || !mma_fits(l, dtype)) return kSimt;
-    return kernel != VC1D_LINEAR_MMA && dtype == VC1D_BF16 && largest_rows(l) <= 160 ? kTc : kMma;
+    return kernel != VC1D_LINEAR_MMA && dtype == VC1D_BF16 && largest_rows(l) <= 160 && tma_fits(l) ? kTc : kMma;
 }
 
 // whether the kernel that the caller names takes this launch
@@ -201,7 +216,7 @@ cudaError_t launch_one(const Launch& l, int dtype, Kind kind, bool states_only, 
 
 // Enqueues the runs of `l`, split along time if the workspace allows it.
 cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, long long ws_bytes, cudaStream_t s) {
-    const Kind kind = pick(l, dtype, kernel);
+    Kind kind = pick(l, dtype, kernel);
     for (int i = 0; i < l.runs; ++i) l.run[i].out_vec = !l.run[i].out_f32 && vector_rows(l.run[i].o, elem_bytes(dtype));
     if (segments > 1 && (ws == nullptr || ws_bytes < split_bytes(l, segments))) segments = 1;
     const int chunks = (l.c.seqlen + chunk_of(kind) - 1) / chunk_of(kind);

@@ -13,12 +13,16 @@
 //     warps 0-3   decays of P, its operand, then the output
 //     warps 4-7   the state: X = a^n X + KV, and its bf16 copy in shared memory   (rows 128-159: warp 14)
 //     warps 8-11  the weighted values, split into three parts
-//     warp 12     issues the products;  warps 13, 15  load tokens (cp.async: masked rows arrive as zeros, unread)
+//     warp 12     issues the products
+//     warp 13     brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
+//     warp 15     clears the rows of masked tokens, whatever they hold, and hands the chunk over
 // While one chunk's P is being decayed, the next chunk's tokens arrive and the state runs ahead.
 //
 // Shared memory holds every operand as panels of 64 channels: rows of 128 bytes with the 16-byte units XORed by the row
 // modulo 8 (the 128-byte swizzle of the matrix descriptors).  A panel serves as K-major (channels summed: q, k) and as
-// MN-major operand (tokens summed: k^T, v, w v; state rows summed: X) alike, so nothing is transposed.
+// MN-major operand (tokens summed: k^T, v, w v; state rows summed: X) alike, so nothing is transposed.  A run from the last
+// token to the first takes its chunks from the end and keeps the tokens of a chunk in their natural order; only the
+// powers of the decay know the direction.
 //
 // Every wait is bounded.  When one expires the CTA notes it (the library's count of expired waits) and gives up.
 #pragma once
@@ -38,7 +42,6 @@ using tma::smem_u32;
 
 constexpr int kC = 128;               // tokens of a chunk
 constexpr int kThreads = 512;
-constexpr int kLoaders = 64;
 constexpr int kPow = kC + 2;          // a^0 .. a^(kC + 1)
 constexpr int kCols = 64;             // columns of a slab
 constexpr int kPanel = kC * 128;      // bytes of a panel of 128 rows
@@ -47,12 +50,18 @@ constexpr unsigned kSpin = 1u << 22;  // polls of 64 ns and more
 // TMEM columns
 constexpr uint32_t kTmP = 0, kTmPb = 128, kTmOi = 192, kTmOa = 256, kTmKV = 320, kTmKV2 = 384, kTmCols = 512;
 
-enum Bar { kFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
+enum Bar { kTma, kFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
 
-struct Info {  // of a chunk's tokens; a ring of four
+struct Info {  // of a chunk's tokens, bit i of word i / 32 for token i; a ring of four
     unsigned valid[4], start[4];
     int n_all, run_all;
-    int n_before[4], run_before[4];  // before each word
+    int n_before[4], run_before[4];  // in the words below
+};
+struct Maps {
+    CUtensorMap a, k, v;
+};
+struct AllMaps {
+    Maps run[kMaxRuns];
 };
 
 template <int ROWS>
@@ -69,13 +78,15 @@ struct Layout {
     static constexpr int kInfo = kAdd + 4 * kC;
     static constexpr int kBar = (kInfo + 4 * (int)sizeof(Info) + 15) & ~15;
     static constexpr int kMisc = kBar + 8 * 2 * kBars;
-    static constexpr int kBytes = kMisc + 16;
+    static constexpr int kBytes = kMisc + 32;
 };
 
 // ---- tcgen05 ----
 __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
+// the same matrix `bytes` further
+__device__ __forceinline__ uint64_t at(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
 // K-major: rows of 128 bytes, groups of 8 rows 1024 bytes apart.  MN-major: 64 elements of a row, the next 64 a panel
 // further; 8 summed rows are 1024 bytes.
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return desc(addr, 16, 1024); }
@@ -119,8 +130,10 @@ __device__ __forceinline__ bool all_of(int id, int threads, bool yes) {
                  : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+                 "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -129,7 +142,7 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 
 // ROWS: state rows the kernel is built for (128 or 160).
 template <int ROWS, bool STATES>
-__global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant__ Launch l, unsigned int* timeouts) {
+__global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant__ Launch l, const __grid_constant__ AllMaps maps, unsigned int* timeouts) {
     using L = Layout<ROWS>;
     using T = __nv_bfloat16;
     constexpr int NS = L::kStages;
@@ -142,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     float* pw_lo = pw_hi + kPow;
     float* add = reinterpret_cast<float*>(sm + L::kAdd);
     Info* infos = reinterpret_cast<Info*>(sm + L::kInfo);
-    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired
+    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4] chunks asked for
     volatile uint32_t* dead = misc + 1;
 
     const Run& r = l.run[blockIdx.z];
@@ -153,9 +166,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     const int b = bh / c.heads, h = bh % c.heads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c0 = slab * kCols, cols = min(kCols, r.dv - c0);
+    const bool rev = r.reverse;
+    // tokens in the run's order; a chunk's first token in natural order, negative where the last chunk of a reversed run
+    // reaches past the first token
     const int t_begin = seg * c.seg_chunks * kC;
     const int t_end = min(c.seqlen, t_begin + c.seg_chunks * kC);
     const int chunks = (t_end - t_begin + kC - 1) / kC;
+    auto first_token = [&](int ch) { return rev ? c.seqlen - t_begin - (ch + 1) * kC : t_begin + ch * kC; };
 
     auto bar = [&](int kind, int chunk) { return base + L::kBar + 8 * (2 * kind + (chunk & 1)); };
     // Waits until the event of `kind` that belongs to `chunk` has happened.  Each kind has two barriers, for even and odd
@@ -185,9 +202,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     }
     for (int i = tid; i < L::kPowers / 16; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
-        misc[1] = 0;
+        misc[1] = misc[4] = 0;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(kFull, i), kLoaders);
+            mbar_init(bar(kTma, i), 1);
+            mbar_init(bar(kFull, i), 32);
             mbar_init(bar(kPRaw, i), 1);
             mbar_init(bar(kPRdy, i), 128);
             mbar_init(bar(kVwRdy, i), 128);
@@ -211,18 +229,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     const uint32_t tm = misc[0];
     const uint32_t tm_lane = tm + ((uint32_t)(warp & 3) << 21);  // a warp reaches the 32 lanes of its place in its group
 
-    // n and run of token i of a chunk, up to and with i
+    // Valid tokens and sequence starts of a chunk up to and with token i, in the run's order.
     auto count = [&](const Info& f, int i, int* n, int* run) {
         const int w = i >> 5;
-        const unsigned upto = 0xffffffffu >> (31 - (i & 31));
-        *n = f.n_before[w] + __popc(f.valid[w] & upto);
-        *run = f.run_before[w] + __popc(f.start[w] & upto);
+        const unsigned upto = 0xffffffffu >> (31 - (i & 31)), below = upto >> 1;
+        *n = rev ? f.n_all - f.n_before[w] - __popc(f.valid[w] & below) : f.n_before[w] + __popc(f.valid[w] & upto);
+        *run = rev ? f.run_all - f.run_before[w] - __popc(f.start[w] & below) : f.run_before[w] + __popc(f.start[w] & upto);
     };
 
     if (warp < 4) {
         // ------------------------------------------------------------------------------ decays of P, output
         const int row = tid;
         const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
+        float pw[32];  // a^31 .. a^0, or a^0 .. a^31
+#pragma unroll
+        for (int j = 0; j < 32; ++j) pw[j] = pw_hi[rev ? j : 31 - j];
         for (int ch = 0; !STATES && ch < chunks; ++ch) {
             if (!wait_warp(kFull, ch) || !wait_warp(kPRaw, ch)) break;
             fence_after();
@@ -236,29 +257,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
 #pragma unroll 1
             for (int blk = 0; blk < 4; ++blk) {  // 32 keys
                 uint32_t p[16];
-                if (blk > warp) {  // later than all queries of this warp
+                if (rev ? blk < warp : blk > warp) {  // later than all queries of this warp
 #pragma unroll
                     for (int j = 0; j < 16; ++j) p[j] = 0;
                 } else {
                     float x[32];
                     tm_ld32(x, tm_lane + kTmP + 32 * blk);
                     tm_wait_ld();
-                    if (plain && blk < warp) {
-                        // a^(row - key) as the product of a power per row and one per key, neither above 1 for a decay
-                        const float own = pw_hi[row - 32 * blk - 31] * r.s_pair;
+                    if (plain && blk != warp) {
+                        // a^|row - key| as the product of a power per row and one per key, neither above 1 for a decay
+                        const float own = pw_hi[rev ? 32 * blk - row : row - 32 * blk - 31] * r.s_pair;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] *= own * pw_hi[31 - j];
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 y = mul2(make_float2(x[j], x[j + 1]), mul2(make_float2(own, own), make_float2(pw[j], pw[j + 1])));
+                            x[j] = y.x, x[j + 1] = y.y;
+                        }
                     } else if (plain) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = j <= lane ? x[j] * (pw_hi[max(lane - j, 0)] * r.s_pair) : 0.f;
+                        for (int j = 0; j < 32; ++j) {
+                            const int lag = rev ? j - lane : lane - j;
+                            x[j] = lag >= 0 ? x[j] * (pw_hi[max(lag, 0)] * r.s_pair) : 0.f;
+                        }
                     } else {
                         const unsigned vb = f.valid[blk], sb = f.start[blk];
                         int n = f.n_before[blk], run = f.run_before[blk];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
+                            const int n0 = n, run0 = run;
                             n += vb >> j & 1u;
                             run += sb >> j & 1u;
-                            const unsigned lag = (unsigned)(code - (n + (run << 8)));
+                            const unsigned lag = (unsigned)(code - (rev ? f.n_all - n0 + ((f.run_all - run0) << 8) : n + (run << 8)));
                             x[j] = lag <= (unsigned)kC ? x[j] * (pw_hi[lag] * r.s_pair) : 0.f;
                         }
                     }
@@ -272,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             mbar_arrive(bar(kPRdy, ch));
             if (!wait_warp(kPvDone, ch)) break;
             fence_after();
-            const int t = t_begin + ch * kC + row;
+            const int t = first_token(ch) + row;
             T* po = const_cast<T*>(static_cast<const T*>(r.o.p)) + obase + (long long)t * r.o.st + c0;
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
@@ -290,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                     const float o = from_x ? fmaf(x[j], carry, y[j]) : y[j];
                     x[j] = ok ? o : 0.f;
                 }
-                if (t < t_end) {
+                if (t >= 0 && t < c.seqlen) {
                     if (r.out_vec) {
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
@@ -444,31 +472,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 if (!wait(kFull, ch)) break;
                 fence_after();
                 if (!STATES) {
-                    for (int s = 0; s < steps; ++s) {
-                        const uint32_t off = (s >> 2) * kPanel + (s & 3) * 32;
-                        mma_ss(tm + kTmP, desc_k(q + off), desc_k(k + off), idesc(128, false, false), s > 0);
-                    }
+                    const uint64_t dq = desc_k(q), dk = desc_k(k);
+#pragma unroll
+                    for (int s = 0; s < ROWS / 16; ++s)
+                        if (s < steps) mma_ss(tm + kTmP, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dk, (s >> 2) * kPanel + (s & 3) * 32), idesc(128, false, false), s > 0);
                     commit(bar(kPRaw, ch));
                 }
                 if (!wait(kVwRdy, ch) || (ch > 0 && !wait(kKvFree, ch - 1))) break;
                 fence_after();
 #pragma unroll 1
-                for (int tile = 0; tile < (kSecond ? 2 : 1); ++tile)  // rows 0-127; 64-191, of which 128-159 are used
+                for (int tile = 0; tile < (kSecond ? 2 : 1); ++tile) {  // rows 0-127; 64-191, of which 128-159 are used
+                    const uint64_t dk = desc_mn(k + tile * kPanel);
+                    uint64_t dw = desc_mn(w0 + 2 * kPanel);
 #pragma unroll 1
-                    for (int p = 2; p >= 0; --p)
-                        for (int s = 0; s < kC / 16; ++s)
-                            mma_ss(tm + (tile ? kTmKV2 : kTmKV), desc_mn(k + tile * kPanel + s * 2048), desc_mn(w0 + p * kPanel + s * 2048),
-                                   idesc(64, true, true), p < 2 || s > 0);
+                    for (int p = 2; p >= 0; --p) {
+#pragma unroll
+                        for (int s = 0; s < kC / 16; ++s) mma_ss(tm + (tile ? kTmKV2 : kTmKV), at(dk, s * 2048), at(dw, s * 2048), idesc(64, true, true), p < 2 || s > 0);
+                        dw -= kPanel >> 4;
+                    }
+                }
                 commit(bar(kKvDone, ch));
                 if (!STATES) {
                     if (!wait(kXRdy, ch) || (ch > 0 && !wait(kOFree, ch - 1))) break;
                     fence_after();
-                    for (int s = 0; s < steps; ++s)
-                        mma_ss(tm + kTmOi, desc_k(q + (s >> 2) * kPanel + (s & 3) * 32), desc_mn(x0 + s * 2048), idesc(64, false, true), s > 0);
+                    const uint64_t dq = desc_k(q), dx = desc_mn(x0), dv = desc_mn(v);
+#pragma unroll
+                    for (int s = 0; s < ROWS / 16; ++s)
+                        if (s < steps) mma_ss(tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(64, false, true), s > 0);
                     commit(bar(kQxDone, ch));
                     if (!wait(kPRdy, ch)) break;
                     fence_after();
-                    for (int s = 0; s < kC / 16; ++s) mma_ts(tm + kTmOa, tm + kTmPb + 8 * s, desc_mn(v + s * 2048), idesc(64, false, true), s > 0);
+#pragma unroll
+                    for (int s = 0; s < kC / 16; ++s) mma_ts(tm + kTmOa, tm + kTmPb + 8 * s, at(dv, s * 2048), idesc(64, false, true), s > 0);
                     commit(bar(kPvDone, ch));
                 }
             }
@@ -476,24 +511,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         __syncwarp();
     } else if (warp != 14) {
         // ------------------------------------------------------------------------------ tokens
-        const int me = (warp == 13 ? 0 : 32) + lane;
-        const T* pa = static_cast<const T*>(r.a.p) + (long long)b * r.a.sb + (long long)(h / r.a.group) * r.a.sh;
-        const T* pk = static_cast<const T*>(r.k.p) + (long long)b * r.k.sb + (long long)(h / r.k.group) * r.k.sh;
-        const T* pv = static_cast<const T*>(r.v.p) + (long long)b * r.v.sb + (long long)(h / r.v.group) * r.v.sh + c0;
-        auto fill_info = [&](int ch) {  // by one warp
+        const Maps& m = maps.run[blockIdx.z];
+        const int panels = (r.da + 63) / 64;
+        for (int ch = 0; warp == 13 && ch < chunks; ++ch) {
+            bool ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
+            ok = ok && (ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2))));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const int t0 = first_token(ch);
+            // the tokens of the chunk that count, and the sequence starts in the run's order
             Info* f = infos + (ch & 3);
-            const int t0 = t_begin + ch * kC;
             int n = 0, run = 0;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const int t = t0 + 32 * w + lane;
-                const long long at = r.reverse ? c.seqlen - 1 - t : t;
-                bool v = t < t_end, s = false;
-                if (v && c.mask != nullptr) v = mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + at * c.mask_st);
-                if (t < t_end && c.seq_idx != nullptr && t > 0) {
-                    const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + at * c.seq_st;
-                    s = p[0] != (r.reverse ? p[c.seq_st] : p[-c.seq_st]);
+                bool v = t >= 0 && t < c.seqlen, s = false;
+                if (v && c.seq_idx != nullptr && (rev ? t + 1 < c.seqlen : t > 0)) {
+                    const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + (long long)t * c.seq_st;
+                    s = p[0] != (rev ? p[c.seq_st] : p[-c.seq_st]);
                 }
+                if (v && c.mask != nullptr) v = mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + (long long)t * c.mask_st);
                 const unsigned vb = __ballot_sync(0xffffffffu, v), sb = __ballot_sync(0xffffffffu, s);
                 if (lane == 0) {
                     f->valid[w] = vb;
@@ -507,65 +543,104 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             if (lane == 0) {
                 f->n_all = n;
                 f->run_all = run;
+                const uint32_t done = bar(kTma, ch);
+                tma::mbar_arrive_expect_tx(done, ((STATES ? 1 : 2) * panels + 1) * kPanel);
+                for (int p = 0; p < panels; ++p) {
+                    tma_load_4d(base + L::kK + ((ch % NS) * L::kPanels + p) * kPanel, &m.k, p * 64, t0, h / r.k.group, b, done);
+                    if (!STATES) tma_load_4d(base + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel, &m.a, p * 64, t0, h / r.a.group, b, done);
+                }
+                tma_load_4d(base + L::kV + (ch & 1) * kPanel, &m.v, c0, t0, h / r.v.group, b, done);
+                misc[4] = ch + 1;
             }
-        };
-        // 16-byte pieces: a thread has the pieces `me & 7` of every eighth row of a panel
-        auto load_panel = [&](const Info& f, const T* src, long long st, bool has, uint32_t dst) {
-            const int u = me & 7;
-#pragma unroll 4
-            for (int row = me >> 3; row < kC; row += kLoaders / 8) {
-                const bool ok = f.valid[row >> 5] >> (row & 31) & 1u;
-                if (has) cp16(dst + row * 128 + ((u ^ (row & 7)) << 4), ok ? src + row * st + u * 8 : src, ok);
-            }
-        };
-        if (warp == 13 && chunks > 0) fill_info(0);
-        for (int ch = 0; ch < chunks; ++ch) {
-            bool ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
-            ok = ok && (ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2))));
-            if (!all_of(2, kLoaders, ok)) break;  // this chunk's info is there
+            __syncwarp();
+        }
+        for (int ch = 0; warp == 15 && ch < chunks; ++ch) {
+            if (!wait_warp(kTma, ch)) break;
             const Info& f = infos[ch & 3];
-            const long long t0 = t_begin + ch * kC;
-            for (int p = 0; p < L::kPanels; ++p) {
-                const bool has = p * 64 + (me & 7) * 8 < r.da;
-                load_panel(f, pk + t0 * r.k.st + p * 64, r.k.st, has, base + L::kK + ((ch % NS) * L::kPanels + p) * kPanel);
-                if (!STATES) load_panel(f, pa + t0 * r.a.st + p * 64, r.a.st, has, base + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel);
+            if (c.mask != nullptr && f.n_all < kC) {
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
+                    if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
+                    const int at = row * 128 + (lane & 7) * 16;
+                    for (int p = 0; p < panels; ++p) {
+                        *reinterpret_cast<uint4*>(sm + L::kK + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
+                        if (!STATES) *reinterpret_cast<uint4*>(sm + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
+                    }
+                    *reinterpret_cast<uint4*>(sm + L::kV + (ch & 1) * kPanel + at) = zero;
+                }
+                fence_async_smem();
             }
-            load_panel(f, pv + t0 * r.v.st, r.v.st, (me & 7) * 8 < cols, base + L::kV + (ch & 1) * kPanel);
-            if (warp == 13 && ch + 1 < chunks) fill_info(ch + 1);
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async_smem();
             mbar_arrive(bar(kFull, ch));
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     fence_before();
     __syncthreads();
     if (warp == 12) {
         fence_after();
         if (*dead && lane == 0) {
-            // products may still be under way: they end by themselves, and TMEM has to outlive them
-            mbar_init(base + L::kBar, 1);
+            // products and copies may still be under way: they end by themselves, and TMEM and shared memory have to
+            // outlive them.  A barrier of its own for the products; the copies' barriers for the copies.
+            const uint32_t last = base + L::kMisc + 8;
+            mbar_init(last, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            commit(base + L::kBar);
-            for (unsigned i = 0; i < kSpin && !mbar_test(base + L::kBar, 0); ++i) __nanosleep(64);
+            commit(last);
+            for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
+            const int issued = misc[4];
+            for (int ch = max(0, issued - 2); ch < issued; ++ch)
+                for (unsigned i = 0; i < kSpin && !mbar_test(bar(kTma, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
         }
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(kTmCols));
     }
 }
 
+// The tensor map of rows as [batch, head, token, channel] with boxes of 64 channels x 128 tokens.
+inline bool encode(CUtensorMap* map, const Rows& r, int batch, int heads, int seqlen, int dim) {
+    tma::EncodeFn enc = tma::encode_fn();
+    if (enc == nullptr) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)seqlen, (cuuint64_t)(heads / r.group), (cuuint64_t)batch};
+    cuuint64_t st[3] = {2 * (cuuint64_t)r.st, 2 * (cuuint64_t)r.sh, 2 * (cuuint64_t)r.sb};
+    for (int i = 0; i < 3; ++i)
+        if (dims[i + 1] == 1) st[i] = 1024;  // an extent of 1 makes its stride irrelevant, but the encoder wants a legal one
+    const cuuint32_t box[4] = {64, kC, 1, 1}, step[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(r.p), dims, st, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// rows whose tokens run backwards, in natural order again
+inline Rows natural(Rows r, int seqlen, int eb) {
+    r.p = static_cast<const char*>(r.p) + (long long)(seqlen - 1) * r.st * eb;
+    r.st = -r.st;
+    return r;
+}
+
 template <int ROWS, bool STATES>
-cudaError_t launch(const Launch& l, unsigned int* timeouts, cudaStream_t s) {
+cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) {
     constexpr int smem = Layout<ROWS>::kBytes + 1008;  // and what aligning the panels takes
     static_assert(smem <= 232448, "shared memory of an SM");
+    Launch l = given;
+    AllMaps maps;
     int slabs = 0;
-    for (int i = 0; i < l.runs; ++i) slabs = max(slabs, (l.run[i].dv + kCols - 1) / kCols);
+    for (int i = 0; i < l.runs; ++i) {
+        Run& r = l.run[i];
+        if (r.reverse) {
+            r.a = natural(r.a, l.c.seqlen, 2);
+            r.k = natural(r.k, l.c.seqlen, 2);
+            r.v = natural(r.v, l.c.seqlen, 2);
+            r.o = natural(r.o, l.c.seqlen, r.out_f32 ? 4 : 2);
+        }
+        slabs = max(slabs, (r.dv + kCols - 1) / kCols);
+        Maps& m = maps.run[i];
+        if (l.c.seqlen > 0 && !(encode(&m.a, r.a, l.c.batch, l.c.heads, l.c.seqlen, r.da) && encode(&m.k, r.k, l.c.batch, l.c.heads, l.c.seqlen, r.da) &&
+                                encode(&m.v, r.v, l.c.batch, l.c.heads, l.c.seqlen, r.dv)))
+            return cudaErrorNotSupported;
+    }
     auto kernel = k_linear_tc<ROWS, STATES>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(l.c.batch * l.c.heads * slabs), STATES ? l.c.segments - 1 : l.c.segments, l.runs);
     note_launch(STATES ? "linear_tc_states" : "linear_tc");
-    kernel<<<grid, kThreads, smem, s>>>(l, timeouts);
+    kernel<<<grid, kThreads, smem, s>>>(l, maps, timeouts);
     return cudaGetLastError();
 }
 

@@ -9,13 +9,16 @@
 //     Oa = bf16(decay P) v          [128 x 64]: P goes back to TMEM as the operand
 // and o = decay Oi + Oa.  The fp32 state stays in registers (a thread per row) and takes each chunk's KV with an fp32
 // multiply-add: the tensor cores never accumulate onto it, because they truncate where an fp32 add rounds.
-// Sixteen warps, each group with its own part, chunk after chunk, linked by mbarriers only:
-//     warps 0-3   decays of P, its operand, then the output
-//     warps 4-7   the state: X = a^n X + KV, and its bf16 copy in shared memory   (rows 128-159: warp 14)
-//     warps 8-11  the weighted values, split into three parts
-//     warp 12     issues the products
-//     warp 13     brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
-//     warp 15     clears the rows of masked tokens, whatever they hold, and hands the chunk over
+// Six groups of four warps, each with its own part, chunk after chunk, linked by mbarriers only:
+//     warps 0-3    decays of P and its operand
+//     warps 4-7    the state: X = a^n X + KV, and its bf16 copy in shared memory   (rows 128-159: warp 22)
+//     warps 8-15   the weighted values, split into three parts
+//     warps 16-19  outputs
+//     warp 20      issues the products
+//     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
+//     warp 23      where there is a mask: clears the rows of masked tokens, whatever they hold, and hands the chunk over
+// The parts are short programs of a few hundred instructions at five or so cycles each, so it is the longest part that
+// sets the pace: that is why there are so many, and twice the warps for the weighted values.
 // While one chunk's P is being decayed, the next chunk's tokens arrive and the state runs ahead.
 //
 // Shared memory holds every operand as panels of 64 channels: rows of 128 bytes with the 16-byte units XORed by the row
@@ -41,7 +44,9 @@ using tma::mbar_test;
 using tma::smem_u32;
 
 constexpr int kC = 128;               // tokens of a chunk
-constexpr int kThreads = 512;
+constexpr int kThreads = 768;
+constexpr int kSmallRegs = 64, kLargeRegs = 112;  // four groups and two: six times the 80 of the launch
+constexpr int kWeighers = 256;
 constexpr int kPow = kC + 2;          // a^0 .. a^(kC + 1)
 constexpr int kCols = 64;             // columns of a slab
 constexpr int kPanel = kC * 128;      // bytes of a panel of 128 rows
@@ -73,7 +78,8 @@ struct Layout {
     static constexpr int kV = kK + kStages * kPanels * kPanel;
     static constexpr int kW = kV + 2 * kPanel;
     static constexpr int kX = kW + 3 * kPanel;
-    static constexpr int kPowers = kX + ROWS * 128;
+    static constexpr int kBlock = kX + ROWS * 128;
+    static constexpr int kPowers = kBlock + 128;
     static constexpr int kAdd = kPowers + 8 * kPow;
     static constexpr int kInfo = kAdd + 4 * kC;
     static constexpr int kBar = (kInfo + 4 * (int)sizeof(Info) + 15) & ~15;
@@ -109,11 +115,28 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The loaded values pass through the wait, so that no use of them can be scheduled before it.
+__device__ __forceinline__ void tm_wait_ld(float (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld(float (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_ld32(float (&r)[32], uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tm_ld16(float (&r)[16], uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
                  : "r"(addr));
 }
 __device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t (&r)[16]) {
@@ -130,6 +153,8 @@ __device__ __forceinline__ bool all_of(int id, int threads, bool yes) {
                  : "memory");
     return r != 0;
 }
+__device__ __forceinline__ void few_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSmallRegs)); }
+__device__ __forceinline__ void many_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kLargeRegs)); }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
                  "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
@@ -140,17 +165,30 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// ROWS: state rows the kernel is built for (128 or 160).
-template <int ROWS, bool STATES>
+// A bounded wait.
+__device__ __forceinline__ bool poll(uint32_t addr, uint32_t parity, volatile uint32_t* dead, unsigned int* timeouts) {
+#pragma unroll 1
+    for (unsigned i = 0; i < kSpin; ++i) {
+        if (mbar_test(addr, parity)) return true;
+        if (*dead) return false;
+        if (i > 64) __nanosleep(64);
+    }
+    *dead = 1;
+    atomicAdd(timeouts, 1u);
+    return false;
+}
+
+// ROWS: state rows the kernel is built for (128 or 160).  REV: tokens run from the last to the first; a constant, because
+// the hot code of all parts together has to stay in the SM's instruction cache.
+template <int ROWS, bool STATES, bool REV>
 __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant__ Launch l, const __grid_constant__ AllMaps maps, unsigned int* timeouts) {
     using L = Layout<ROWS>;
     using T = __nv_bfloat16;
     constexpr int NS = L::kStages;
     constexpr bool kSecond = ROWS > 128;  // warp 14 holds rows 128 and up
-    extern __shared__ unsigned char raw[];
-    // the swizzle goes by address: panels start at multiples of 1024
-    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-    unsigned char* sm = raw + (base - smem_u32(raw));
+    extern __shared__ __align__(1024) unsigned char sm[];  // the swizzle goes by address: panels start at multiples of 1024
+    const uint32_t base = smem_u32(sm);
+    float* block = reinterpret_cast<float*>(sm + L::kBlock);  // a^31 .. a^0; a^0 .. a^31 in a reversed run
     float* pw_hi = reinterpret_cast<float*>(sm + L::kPowers);
     float* pw_lo = pw_hi + kPow;
     float* add = reinterpret_cast<float*>(sm + L::kAdd);
@@ -163,10 +201,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     const int slabs = (r.dv + kCols - 1) / kCols;
     const int slab = blockIdx.x % slabs, bh = blockIdx.x / slabs, seg = blockIdx.y;
     if (bh >= c.batch * c.heads) return;  // a run with fewer slabs than the launch's widest
+    if ((base & 1023u) != 0) {  // cannot be: the array says so
+        if (threadIdx.x == 0) atomicAdd(timeouts, 1u);
+        return;
+    }
     const int b = bh / c.heads, h = bh % c.heads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int c0 = slab * kCols, cols = min(kCols, r.dv - c0);
-    const bool rev = r.reverse;
+    constexpr bool rev = REV;
     // tokens in the run's order; a chunk's first token in natural order, negative where the last chunk of a reversed run
     // reaches past the first token
     const int t_begin = seg * c.seg_chunks * kC;
@@ -177,18 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     auto bar = [&](int kind, int chunk) { return base + L::kBar + 8 * (2 * kind + (chunk & 1)); };
     // Waits until the event of `kind` that belongs to `chunk` has happened.  Each kind has two barriers, for even and odd
     // chunks: nobody who waits is ever two chunks behind, so a phase cannot be missed.
-    auto wait = [&](int kind, int chunk) {
-        const uint32_t addr = bar(kind, chunk), parity = (uint32_t)(chunk >> 1) & 1u;
-        for (unsigned i = 0; i < kSpin; ++i) {
-            if (mbar_test(addr, parity)) return true;
-            if (*dead) return false;
-            if (i > 64) __nanosleep(64);
-        }
-        *dead = 1;
-        atomicAdd(timeouts, 1u);
-        return false;
-    };
-
+    auto wait = [&](int kind, int chunk) { return poll(bar(kind, chunk), (uint32_t)(chunk >> 1) & 1u, dead, timeouts); };
     // by a whole warp, with one answer for all of it
     auto wait_warp = [&](int kind, int chunk) { return (bool)__all_sync(0xffffffffu, wait(kind, chunk)); };
 
@@ -199,16 +230,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         const double lo = x - (double)hi;
         pw_hi[n] = hi;
         pw_lo[n] = (isfinite(hi) && lo == lo) ? (float)lo : 0.f;
+        if (n < 32) block[rev ? n : 31 - n] = hi;
     }
-    for (int i = tid; i < L::kPowers / 16; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < L::kBlock / 16; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
         misc[1] = misc[4] = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(kTma, i), 1);
-            mbar_init(bar(kFull, i), 32);
+            mbar_init(bar(kFull, i), c.mask != nullptr ? 32 : 1);
             mbar_init(bar(kPRaw, i), 1);
             mbar_init(bar(kPRdy, i), 128);
-            mbar_init(bar(kVwRdy, i), 128);
+            mbar_init(bar(kVwRdy, i), kWeighers);
             mbar_init(bar(kKvDone, i), 1);
             mbar_init(bar(kKvFree, i), kSecond ? 160 : 128);
             mbar_init(bar(kXRdy, i), kSecond ? 160 : 128);
@@ -218,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(misc)), "n"(kTmCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -237,125 +269,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         *run = rev ? f.run_all - f.run_before[w] - __popc(f.start[w] & below) : f.run_before[w] + __popc(f.start[w] & upto);
     };
 
-    if (warp < 4) {
-        // ------------------------------------------------------------------------------ decays of P, output
-        const int row = tid;
-        const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
-        float pw[32];  // a^31 .. a^0, or a^0 .. a^31
-#pragma unroll
-        for (int j = 0; j < 32; ++j) pw[j] = pw_hi[rev ? j : 31 - j];
-        for (int ch = 0; !STATES && ch < chunks; ++ch) {
-            if (!wait_warp(kFull, ch) || !wait_warp(kPRaw, ch)) break;
-            fence_after();
-            const Info& f = infos[ch & 3];
-            int n_i, run_i;
-            count(f, row, &n_i, &run_i);
-            const int code = n_i + (run_i << 8);
-            const bool ok = f.valid[warp] >> lane & 1u, from_x = run_i == 0;
-            const float carry = pw_hi[max(n_i - r.shift, 0)] * r.s_carry;
-            const bool plain = f.n_all == kC && f.run_all == 0;  // every token valid, one sequence
-#pragma unroll 1
-            for (int blk = 0; blk < 4; ++blk) {  // 32 keys
-                uint32_t p[16];
-                if (rev ? blk < warp : blk > warp) {  // later than all queries of this warp
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) p[j] = 0;
-                } else {
-                    float x[32];
-                    tm_ld32(x, tm_lane + kTmP + 32 * blk);
-                    tm_wait_ld();
-                    if (plain && blk != warp) {
-                        // a^|row - key| as the product of a power per row and one per key, neither above 1 for a decay
-                        const float own = pw_hi[rev ? 32 * blk - row : row - 32 * blk - 31] * r.s_pair;
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float2 y = mul2(make_float2(x[j], x[j + 1]), mul2(make_float2(own, own), make_float2(pw[j], pw[j + 1])));
-                            x[j] = y.x, x[j + 1] = y.y;
-                        }
-                    } else if (plain) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int lag = rev ? j - lane : lane - j;
-                            x[j] = lag >= 0 ? x[j] * (pw_hi[max(lag, 0)] * r.s_pair) : 0.f;
-                        }
-                    } else {
-                        const unsigned vb = f.valid[blk], sb = f.start[blk];
-                        int n = f.n_before[blk], run = f.run_before[blk];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int n0 = n, run0 = run;
-                            n += vb >> j & 1u;
-                            run += sb >> j & 1u;
-                            const unsigned lag = (unsigned)(code - (rev ? f.n_all - n0 + ((f.run_all - run0) << 8) : n + (run << 8)));
-                            x[j] = lag <= (unsigned)kC ? x[j] * (pw_hi[lag] * r.s_pair) : 0.f;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) p[j] = pack(x[2 * j], x[2 * j + 1]);
-                }
-                tm_st16(tm_lane + kTmPb + 16 * blk, p);
-            }
-            tm_wait_st();
-            fence_before();
-            mbar_arrive(bar(kPRdy, ch));
-            if (!wait_warp(kPvDone, ch)) break;
-            fence_after();
-            const int t = first_token(ch) + row;
-            T* po = const_cast<T*>(static_cast<const T*>(r.o.p)) + obase + (long long)t * r.o.st + c0;
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                float x[32], y[32];
-                tm_ld32(x, tm_lane + kTmOi + 32 * half);
-                tm_ld32(y, tm_lane + kTmOa + 32 * half);
-                tm_wait_ld();
-                if (half == 1) {
-                    fence_before();
-                    mbar_arrive(bar(kOFree, ch));
-                }
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    // a later sequence takes nothing of X, infinities neither
-                    const float o = from_x ? fmaf(x[j], carry, y[j]) : y[j];
-                    x[j] = ok ? o : 0.f;
-                }
-                if (t >= 0 && t < c.seqlen) {
-                    if (r.out_vec) {
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (32 * half + 8 * u < cols)
-                                st_vec(po + 32 * half + 8 * u, make_uint4(pack(x[8 * u], x[8 * u + 1]), pack(x[8 * u + 2], x[8 * u + 3]),
-                                                                          pack(x[8 * u + 4], x[8 * u + 5]), pack(x[8 * u + 6], x[8 * u + 7])));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int col = 32 * half + j;
-                            if (col < cols) {
-                                const long long at = obase + (long long)t * r.o.st + (long long)(c0 + col) * r.o.sd;
-                                if (r.out_f32)
-                                    const_cast<float*>(static_cast<const float*>(r.o.p))[at] = x[j];
-                                else
-                                    const_cast<T*>(static_cast<const T*>(r.o.p))[at] = __float2bfloat16_rn(x[j]);
-                            }
-                        }
-                    }
-                }
-            }
-        }
-    } else if (warp < 8 || (kSecond && warp == 14)) {
-        // ------------------------------------------------------------------------------ state
-        const int row = (warp == 14 ? 128 : 32 * (warp - 4)) + lane;
-        const uint32_t kv = tm_lane + (warp == 14 ? kTmKV2 : kTmKV);
+    // The part of the warps that hold the state, a thread per row; its sums are in the TMEM columns from `column` on.
+    auto state = [&](int row, uint32_t column) {
+        const uint32_t kv = tm_lane + column;
         float X[kCols];
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-            float x = 0.f;
-            if (!STATES && row < r.da && j < cols) {
-                if (seg > 0)
-                    x = c.seg_state[blockIdx.z][((long long)(seg - 1) * c.batch * c.heads + bh) * ((long long)r.da * r.dv) + (long long)row * r.dv + c0 + j];
-                else if (r.x0.p != nullptr)
-                    x = r.x0.p[(long long)b * r.x0.sb + (long long)h * r.x0.sh + (long long)row * r.x0.sr + (long long)(c0 + j) * r.x0.sc];
+        {
+            const float* src = nullptr;
+            long long step = 1;
+            if (!STATES && row < r.da) {
+                if (seg > 0) {
+                    src = c.seg_state[blockIdx.z] + ((long long)(seg - 1) * c.batch * c.heads + bh) * ((long long)r.da * r.dv) + (long long)row * r.dv + c0;
+                } else if (r.x0.p != nullptr) {
+                    src = r.x0.p + (long long)b * r.x0.sb + (long long)h * r.x0.sh + (long long)row * r.x0.sr + (long long)c0 * r.x0.sc;
+                    step = r.x0.sc;
+                }
             }
-            X[j] = x;
+            const int n = src == nullptr ? 0 : cols;
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) {
+                X[j] = j < n ? *src : 0.f;
+                src += step;
+            }
         }
         auto store_x = [&]() {
             unsigned char* p = sm + L::kX + row * 128;
@@ -371,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         }
         double seg_factor = 1.0;
         bool fine = true;
+#pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
             if (!wait_warp(kFull, ch) || !wait_warp(kKvDone, ch)) {
                 fine = false;
@@ -382,17 +317,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             const bool keep = f.run_all == 0;
             if (STATES) seg_factor = keep ? seg_factor * ((double)fac.x + (double)fac.y) : 0.0;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float x[32];
-                tm_ld32(x, kv + 32 * half);
-                tm_wait_ld();
-                if (half == 1) {
+            for (int j0 = 0; j0 < kCols; j0 += 16) {
+                float x[16];
+                tm_ld16(x, kv + j0);
+                tm_wait_ld(x);
+                if (j0 + 16 == kCols) {
                     fence_before();
                     mbar_arrive(bar(kKvFree, ch));
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    float* s = X + 32 * half + j;
+                for (int j = 0; j < 16; j += 2) {
+                    float* s = X + j0 + j;
                     float2 y = make_float2(x[j], x[j + 1]);
                     if (keep) y = fma2(make_float2(s[0], s[1]), make_float2(fac.x, fac.x), fma2(make_float2(s[0], s[1]), make_float2(fac.y, fac.y), y));
                     s[0] = y.x;
@@ -412,33 +347,166 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             float* dst = STATES ? c.seg_state[blockIdx.z] + ((long long)seg * c.batch * c.heads + bh) * ((long long)r.da * r.dv) + (long long)row * r.dv
                                 : r.xT.p + (long long)b * r.xT.sb + (long long)h * r.xT.sh + (long long)row * r.xT.sr;
             const long long sc = STATES ? 1 : r.xT.sc;
+            dst += c0 * sc;
 #pragma unroll
-            for (int j = 0; j < kCols; ++j)
-                if (j < cols) dst[(long long)(c0 + j) * sc] = X[j];
+            for (int j = 0; j < kCols; ++j) {
+                if (j < cols) *dst = X[j];
+                dst += sc;
+            }
             if (STATES && slab == 0 && row == 0) {
                 const float hi = (float)seg_factor;
                 c.seg_factor[blockIdx.z][(long long)seg * c.batch * c.heads + bh] = make_float2(hi, (float)(seg_factor - (double)hi));
             }
         }
-    } else if (warp < 12) {
+    };
+
+    if (warp < 4) {
+        // ------------------------------------------------------------------------------ decays of P
+        few_registers();
+        const int row = tid;
+#pragma unroll 1
+        for (int ch = 0; !STATES && ch < chunks; ++ch) {
+            // the products that read the operand of the chunk before have to be done with it
+            if (!wait_warp(kFull, ch) || !wait_warp(kPRaw, ch) || (ch > 0 && !wait_warp(kPvDone, ch - 1))) break;
+            fence_after();
+            const Info& f = infos[ch & 3];
+            const bool plain = f.n_all == kC && f.run_all == 0;  // every token valid, one sequence
+#pragma unroll 1
+            for (int blk = 0; blk < 4; ++blk) {  // 32 keys
+                uint32_t p[16];
+                if (rev ? blk < warp : blk > warp) {  // later than all queries of this warp
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) p[j] = 0;
+                } else {
+                    float x[32];
+                    tm_ld32(x, tm_lane + kTmP + 32 * blk);
+                    tm_wait_ld(x);
+                    if (plain && blk != warp) {
+                        // a^|row - key| as the product of a power per row and one per key, neither above 1 for a decay
+                        const float own = pw_hi[rev ? 32 * blk - row : row - 32 * blk - 31] * r.s_pair;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 w = *reinterpret_cast<const float4*>(block + j);
+                            const float2 y = mul2(make_float2(x[j], x[j + 1]), mul2(make_float2(own, own), make_float2(w.x, w.y)));
+                            const float2 z = mul2(make_float2(x[j + 2], x[j + 3]), mul2(make_float2(own, own), make_float2(w.z, w.w)));
+                            p[j / 2] = pack(y.x, y.y);
+                            p[j / 2 + 1] = pack(z.x, z.y);
+                        }
+                    } else if (plain) {
+                        const float* pz = pw_hi + (rev ? -lane : lane);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            // negative lags are later tokens; their powers are read at 0 and not used
+                            const int l0 = rev ? j - lane : lane - j, l1 = rev ? l0 + 1 : l0 - 1;
+                            const float y = l0 >= 0 ? x[j] * (pz[rev ? j : -j] * r.s_pair) : 0.f;
+                            const float z = l1 >= 0 ? x[j + 1] * (pz[rev ? j + 1 : -j - 1] * r.s_pair) : 0.f;
+                            p[j / 2] = pack(y, z);
+                        }
+                    } else {
+                        int n_i, run_i;
+                        count(f, row, &n_i, &run_i);
+                        const int code = n_i + (run_i << 8);
+                        const unsigned vb = f.valid[blk], sb = f.start[blk];
+                        int n = f.n_before[blk], run = f.run_before[blk];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int n0 = n, run0 = run;
+                            n += vb >> j & 1u;
+                            run += sb >> j & 1u;
+                            const unsigned lag = (unsigned)(code - (rev ? f.n_all - n0 + ((f.run_all - run0) << 8) : n + (run << 8)));
+                            x[j] = lag <= (unsigned)kC ? x[j] * (pw_hi[lag] * r.s_pair) : 0.f;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) p[j] = pack(x[2 * j], x[2 * j + 1]);
+                    }
+                }
+                tm_st16(tm_lane + kTmPb + 16 * blk, p);
+            }
+            tm_wait_st();
+            fence_before();
+            mbar_arrive(bar(kPRdy, ch));
+        }
+    } else if (warp >= 16 && warp < 20) {
+        // ------------------------------------------------------------------------------ outputs
+        few_registers();
+        const int row = tid - 512;
+        const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
+#pragma unroll 1
+        for (int ch = 0; !STATES && ch < chunks; ++ch) {
+            if (!wait_warp(kPvDone, ch)) break;
+            fence_after();
+            const Info& f = infos[ch & 3];
+            int n_i, run_i;
+            count(f, row, &n_i, &run_i);
+            const bool ok = f.valid[warp & 3] >> lane & 1u, from_x = run_i == 0;
+            const float carry = pw_hi[max(n_i - r.shift, 0)] * r.s_carry;
+            const int t = first_token(ch) + row;
+            T* po = const_cast<T*>(static_cast<const T*>(r.o.p)) + obase + (long long)t * r.o.st + c0;
+#pragma unroll 1
+            for (int j0 = 0; j0 < kCols; j0 += 16) {
+                float x[16], y[16];
+                tm_ld16(x, tm_lane + kTmOi + j0);
+                tm_ld16(y, tm_lane + kTmOa + j0);
+                tm_wait_ld(x);
+                tm_wait_ld(y);
+                if (j0 + 16 == kCols) {
+                    fence_before();
+                    mbar_arrive(bar(kOFree, ch));
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    // a later sequence takes nothing of X, infinities neither
+                    const float o = from_x ? fmaf(x[j], carry, y[j]) : y[j];
+                    x[j] = ok ? o : 0.f;
+                }
+                if (t >= 0 && t < c.seqlen) {
+                    if (r.out_vec) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (j0 + 8 * u < cols)
+                                st_vec(po + j0 + 8 * u, make_uint4(pack(x[8 * u], x[8 * u + 1]), pack(x[8 * u + 2], x[8 * u + 3]),
+                                                                   pack(x[8 * u + 4], x[8 * u + 5]), pack(x[8 * u + 6], x[8 * u + 7])));
+                    } else {
+const int eb = r.out_f32 ? 4 : 2;
+                        char* q = const_cast<char*>(static_cast<const char*>(r.o.p)) + (obase + (long long)t * r.o.st + (c0 + j0) * r.o.sd) * eb;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            if (j0 + j < cols) {
+                                if (r.out_f32)
+                                    *reinterpret_cast<float*>(q) = x[j];
+                                else
+                                    *reinterpret_cast<T*>(q) = __float2bfloat16_rn(x[j]);
+                            }
+                            q += r.o.sd * eb;
+                        }
+                    }
+                }
+            }
+        }
+    } else if (warp < 8) {
+        many_registers();
+        state(32 * (warp - 4) + lane, kTmKV);
+    } else if (warp < 16) {
         // ------------------------------------------------------------------------------ weighted values
+        few_registers();
         const int me = tid - 256;
+#pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
             const bool ok = wait(kFull, ch) && (ch == 0 || wait(kKvDone, ch - 1));
-            if (!all_of(1, 128, ok)) break;  // the weights of the chunk before are no longer read
+            if (!all_of(1, kWeighers, ok)) break;  // the weights of the chunk before are no longer read
             const Info& f = infos[ch & 3];
-            {
+            if (me < kC) {
                 int n, run;
                 count(f, me, &n, &run);
                 add[me] = run == f.run_all ? pw_hi[f.n_all - n + r.shift] * r.s_add : 0.f;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
             }
+            asm volatile("bar.sync 1, %0;" ::"n"(kWeighers) : "memory");
             const unsigned char* v = sm + L::kV + (ch & 1) * kPanel;
             unsigned char* w = sm + L::kW;
-            const int at = ((me & 7) ^ (me >> 3 & 7)) << 4;  // rows 16 apart have the same swizzle
+            const int at = ((me & 7) ^ (me >> 3 & 7)) << 4;  // rows 32 apart have the same swizzle
 #pragma unroll 2
-            for (int i = 0; i < 8; ++i) {
-                const int tok = (me >> 3) + 16 * i;
+            for (int i = 0; i < kC * 8 / kWeighers; ++i) {
+                const int tok = (me >> 3) + kWeighers / 8 * i;
                 const uint4 in = *reinterpret_cast<const uint4*>(v + tok * 128 + at);
                 const float2 wt = make_float2(add[tok], add[tok]);
                 const uint32_t e[4] = {in.x, in.y, in.z, in.w};
@@ -462,12 +530,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             fence_async_smem();
             mbar_arrive(bar(kVwRdy, ch));
         }
-    } else if (warp == 12) {
+    } else {
+        many_registers();  // the same instruction for the four warps of the group
         // ------------------------------------------------------------------------------ products
-        if (lane == 0) {
+        if (warp == 20 && lane == 0) {
             const int steps = (r.da + 15) / 16;
             const uint32_t q0 = base + L::kQ, k0 = base + L::kK, v0 = base + L::kV, w0 = base + L::kW, x0 = base + L::kX;
-            for (int ch = 0; ch < chunks; ++ch) {
+    #pragma unroll 1
+        for (int ch = 0; ch < chunks; ++ch) {
                 const uint32_t q = q0 + (ch % NS) * L::kPanels * kPanel, k = k0 + (ch % NS) * L::kPanels * kPanel, v = v0 + (ch & 1) * kPanel;
                 if (!wait(kFull, ch)) break;
                 fence_after();
@@ -508,15 +578,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 }
             }
         }
-        __syncwarp();
-    } else if (warp != 14) {
+        if (kSecond && warp == 22) state(128 + lane, kTmKV2);
         // ------------------------------------------------------------------------------ tokens
         const Maps& m = maps.run[blockIdx.z];
         const int panels = (r.da + 63) / 64;
-        for (int ch = 0; warp == 13 && ch < chunks; ++ch) {
-            bool ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
-            ok = ok && (ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2))));
-            if (!__all_sync(0xffffffffu, ok)) break;
+        const int head_a = h / r.a.group, head_k = h / r.k.group, head_v = h / r.v.group;
+#pragma unroll 1
+        for (int ch = 0; warp == 21 && ch < chunks; ++ch) {
             const int t0 = first_token(ch);
             // the tokens of the chunk that count, and the sequence starts in the run's order
             Info* f = infos + (ch & 3);
@@ -540,24 +608,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 n += __popc(vb);
                 run += __popc(sb);
             }
+            // the buffers are free
+            bool ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
+            ok = ok && (ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2))));
+            if (!__all_sync(0xffffffffu, ok)) break;
             if (lane == 0) {
                 f->n_all = n;
                 f->run_all = run;
-                const uint32_t done = bar(kTma, ch);
+                const uint32_t done = bar(c.mask != nullptr ? kTma : kFull, ch);
                 tma::mbar_arrive_expect_tx(done, ((STATES ? 1 : 2) * panels + 1) * kPanel);
                 for (int p = 0; p < panels; ++p) {
-                    tma_load_4d(base + L::kK + ((ch % NS) * L::kPanels + p) * kPanel, &m.k, p * 64, t0, h / r.k.group, b, done);
-                    if (!STATES) tma_load_4d(base + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel, &m.a, p * 64, t0, h / r.a.group, b, done);
+                    tma_load_4d(base + L::kK + ((ch % NS) * L::kPanels + p) * kPanel, &m.k, p * 64, t0, head_k, b, done);
+                    if (!STATES) tma_load_4d(base + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel, &m.a, p * 64, t0, head_a, b, done);
                 }
-                tma_load_4d(base + L::kV + (ch & 1) * kPanel, &m.v, c0, t0, h / r.v.group, b, done);
+                tma_load_4d(base + L::kV + (ch & 1) * kPanel, &m.v, c0, t0, head_v, b, done);
                 misc[4] = ch + 1;
             }
             __syncwarp();
         }
-        for (int ch = 0; warp == 15 && ch < chunks; ++ch) {
+#pragma unroll 1
+        for (int ch = 0; warp == 23 && c.mask != nullptr && ch < chunks; ++ch) {
             if (!wait_warp(kTma, ch)) break;
             const Info& f = infos[ch & 3];
-            if (c.mask != nullptr && f.n_all < kC) {
+            if (f.n_all < kC) {
                 const uint4 zero = make_uint4(0, 0, 0, 0);
                 for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
                     if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
@@ -573,9 +646,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             mbar_arrive(bar(kFull, ch));
         }
     }
+    __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         fence_after();
         if (*dead && lane == 0) {
             // products and copies may still be under way: they end by themselves, and TMEM and shared memory have to
@@ -587,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
             const int issued = misc[4];
             for (int ch = max(0, issued - 2); ch < issued; ++ch)
-                for (unsigned i = 0; i < kSpin && !mbar_test(bar(kTma, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+                for (unsigned i = 0; i < kSpin && !mbar_test(bar(c.mask != nullptr ? kTma : kFull, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
         }
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(kTmCols));
@@ -614,9 +688,9 @@ inline Rows natural(Rows r, int seqlen, int eb) {
     return r;
 }
 
-template <int ROWS, bool STATES>
+template <int ROWS, bool STATES, bool REV>
 cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) {
-    constexpr int smem = Layout<ROWS>::kBytes + 1008;  // and what aligning the panels takes
+    constexpr int smem = Layout<ROWS>::kBytes;
     static_assert(smem <= 232448, "shared memory of an SM");
     Launch l = given;
     AllMaps maps;
@@ -635,7 +709,7 @@ cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) 
                                 encode(&m.v, r.v, l.c.batch, l.c.heads, l.c.seqlen, r.dv)))
             return cudaErrorNotSupported;
     }
-    auto kernel = k_linear_tc<ROWS, STATES>;
+    auto kernel = k_linear_tc<ROWS, STATES, REV>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(l.c.batch * l.c.heads * slabs), STATES ? l.c.segments - 1 : l.c.segments, l.runs);

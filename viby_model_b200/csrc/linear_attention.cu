@@ -199,9 +199,16 @@ int plan_launch(const Launch& l, int dtype, int kernel, int wanted) {
     for (int i = 0; i < l.runs; ++i) ctas += (long long)l.c.batch * l.c.heads * ((l.run[i].dv + slab - 1) / slab);
     int n = wanted;
     if (n == 0) {
-        // no more CTAs than run at once; a part costs its keys and values once more, so it is at least 256 tokens
-        const long long full = (long long)ctas_per_sm(l, kind) * sm_count();
-        n = ctas >= sm_count() ? 1 : (int)std::min<long long>(full / std::max(1LL, ctas), std::max(1, l.c.seqlen / 256));
+        // Time in units of a chunk: waves of CTAs, each of them its chunks and a start-up of one and a half; a split adds
+        // the pass over keys and values that finds the parts' states (half a chunk's work) and the join.
+        const long long slots = (long long)ctas_per_sm(l, kind) * sm_count();
+        double best = 0;
+        for (int m = 1; m <= std::min(kMaxSegments, std::max(1, l.c.seqlen / 256)); ++m) {
+            const double per = (chunks + m - 1) / m;
+            double t = (double)((ctas * m + slots - 1) / slots) * (per + 1.5);
+            if (m > 1) t += (double)((ctas * (m - 1) + slots - 1) / slots) * (0.5 * per + 1.5) + 1.5;
+            if (m == 1 || t < best) best = t, n = m;
+        }
     }
     n = std::max(1, std::min({n, kMaxSegments, chunks}));
     const int per = (chunks + n - 1) / n;

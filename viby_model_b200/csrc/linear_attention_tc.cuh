@@ -10,10 +10,10 @@
 // and o = decay Oi + Oa.  The fp32 state stays in registers (a thread per row) and takes each chunk's KV with an fp32
 // multiply-add: the tensor cores never accumulate onto it, because they truncate where an fp32 add rounds.
 // Six groups of four warps, each with its own part, chunk after chunk, linked by mbarriers only:
-//     warps 0-3    decays of P and its operand
+//     warps 0-3    decays of P and its operand for the keys 0-63, then the columns 0-31 of the output
 //     warps 4-7    the state: X = a^n X + KV, and its bf16 copy in shared memory   (rows 128-159: warp 22)
 //     warps 8-15   the weighted values, split into three parts
-//     warps 16-19  outputs
+//     warps 16-19  the same for the keys 64-127 and the columns 32-63
 //     warp 20      issues the products
 //     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
 //     warp 23      where there is a mask: clears the rows of masked tokens, whatever they hold, and hands the chunk over
@@ -53,7 +53,11 @@ constexpr int kPanel = kC * 128;      // bytes of a panel of 128 rows
 constexpr unsigned kSpin = 1u << 22;  // polls of 64 ns and more
 
 // TMEM columns
-constexpr uint32_t kTmP = 0, kTmPb = 128, kTmOi = 192, kTmOa = 256, kTmKV = 320, kTmKV2 = 384, kTmCols = 512;
+// P has two buffers, for even and odd chunks, so that the next chunk's products need not wait for this one's decays.  The
+// operand made from P takes P's place: keys 0-63 in columns 0-31, keys 64-127 in columns 64-95, each over products that
+// the warps which write it have read themselves.
+constexpr uint32_t kTmP = 0, kTmOi = 256, kTmOa = 320, kTmKV = 384, kTmKV2 = 448, kTmCols = 512;
+__host__ __device__ constexpr uint32_t operand_column(int blk) { return (blk >> 1) * 64 + (blk & 1) * 16; }  // of 32 keys
 
 enum Bar { kTma, kFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
 
@@ -79,7 +83,7 @@ struct Layout {
     static constexpr int kW = kV + 2 * kPanel;
     static constexpr int kX = kW + 3 * kPanel;
     static constexpr int kBlock = kX + ROWS * 128;
-    static constexpr int kPowers = kBlock + 128;
+    static constexpr int kPowers = kBlock + 256;  // 32 zeros before them
     static constexpr int kAdd = kPowers + 8 * kPow;
     static constexpr int kInfo = kAdd + 4 * kC;
     static constexpr int kBar = (kInfo + 4 * (int)sizeof(Info) + 15) & ~15;
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         const double lo = x - (double)hi;
         pw_hi[n] = hi;
         pw_lo[n] = (isfinite(hi) && lo == lo) ? (float)lo : 0.f;
-        if (n < 32) block[rev ? n : 31 - n] = hi;
+        if (n < 32) block[rev ? n : 31 - n] = hi, pw_hi[n - 32] = 0.f;
     }
     for (int i = tid; i < L::kBlock / 16; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
@@ -239,14 +243,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             mbar_init(bar(kTma, i), 1);
             mbar_init(bar(kFull, i), c.mask != nullptr ? 32 : 1);
             mbar_init(bar(kPRaw, i), 1);
-            mbar_init(bar(kPRdy, i), 128);
+            mbar_init(bar(kPRdy, i), 256);
             mbar_init(bar(kVwRdy, i), kWeighers);
             mbar_init(bar(kKvDone, i), 1);
             mbar_init(bar(kKvFree, i), kSecond ? 160 : 128);
             mbar_init(bar(kXRdy, i), kSecond ? 160 : 128);
             mbar_init(bar(kQxDone, i), 1);
             mbar_init(bar(kPvDone, i), 1);
-            mbar_init(bar(kOFree, i), 128);
+            mbar_init(bar(kOFree, i), 256);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -360,28 +364,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         }
     };
 
-    if (warp < 4) {
-        // ------------------------------------------------------------------------------ decays of P
+    if (warp < 4 || (warp >= 16 && warp < 20)) {
+        // ------------------------------------------------------------------------------ decays of P, outputs
         few_registers();
-        const int row = tid;
+        const int half = warp >> 4, place = warp & 3, row = 32 * place + lane;
+        const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
 #pragma unroll 1
         for (int ch = 0; !STATES && ch < chunks; ++ch) {
-            // the products that read the operand of the chunk before have to be done with it
-            if (!wait_warp(kFull, ch) || !wait_warp(kPRaw, ch) || (ch > 0 && !wait_warp(kPvDone, ch - 1))) break;
+            if (!wait_warp(kFull, ch) || !wait_warp(kPRaw, ch)) break;
             fence_after();
+            const uint32_t tm_p = tm_lane + kTmP + (ch & 1) * 128;
             const Info& f = infos[ch & 3];
+            int n_i, run_i;
+            count(f, row, &n_i, &run_i);
             const bool plain = f.n_all == kC && f.run_all == 0;  // every token valid, one sequence
 #pragma unroll 1
-            for (int blk = 0; blk < 4; ++blk) {  // 32 keys
+            for (int blk = 2 * half; blk < 2 * half + 2; ++blk) {  // 32 keys
                 uint32_t p[16];
-                if (rev ? blk < warp : blk > warp) {  // later than all queries of this warp
+                if (rev ? blk < place : blk > place) {  // later than all queries of this warp
 #pragma unroll
                     for (int j = 0; j < 16; ++j) p[j] = 0;
                 } else {
                     float x[32];
-                    tm_ld32(x, tm_lane + kTmP + 32 * blk);
+                    tm_ld32(x, tm_p + 32 * blk);
                     tm_wait_ld(x);
-                    if (plain && blk != warp) {
+                    if (plain && blk != place) {
                         // a^|row - key| as the product of a power per row and one per key, neither above 1 for a decay
                         const float own = pw_hi[rev ? 32 * blk - row : row - 32 * blk - 31] * r.s_pair;
 #pragma unroll
@@ -393,18 +400,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                             p[j / 2 + 1] = pack(z.x, z.y);
                         }
                     } else if (plain) {
-                        const float* pz = pw_hi + (rev ? -lane : lane);
+                        const float* pz = pw_hi + (rev ? -lane : lane);  // 32 zeros lie before the powers, for later tokens
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            // negative lags are later tokens; their powers are read at 0 and not used
-                            const int l0 = rev ? j - lane : lane - j, l1 = rev ? l0 + 1 : l0 - 1;
-                            const float y = l0 >= 0 ? x[j] * (pz[rev ? j : -j] * r.s_pair) : 0.f;
-                            const float z = l1 >= 0 ? x[j + 1] * (pz[rev ? j + 1 : -j - 1] * r.s_pair) : 0.f;
-                            p[j / 2] = pack(y, z);
+                        for (int j = 0; j < 32; ++j) {
+                            const float y = x[j] * (pz[rev ? j : -j] * r.s_pair);
+                            x[j] = (rev ? j >= lane : j <= lane) ? y : 0.f;  // whatever they hold
                         }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) p[j] = pack(x[2 * j], x[2 * j + 1]);
                     } else {
-                        int n_i, run_i;
-                        count(f, row, &n_i, &run_i);
                         const int code = n_i + (run_i << 8);
                         const unsigned vb = f.valid[blk], sb = f.start[blk];
                         int n = f.n_before[blk], run = f.run_before[blk];
@@ -420,36 +424,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                         for (int j = 0; j < 16; ++j) p[j] = pack(x[2 * j], x[2 * j + 1]);
                     }
                 }
-                tm_st16(tm_lane + kTmPb + 16 * blk, p);
+                tm_st16(tm_p + operand_column(blk), p);
             }
             tm_wait_st();
             fence_before();
             mbar_arrive(bar(kPRdy, ch));
-        }
-    } else if (warp >= 16 && warp < 20) {
-        // ------------------------------------------------------------------------------ outputs
-        few_registers();
-        const int row = tid - 512;
-        const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
-#pragma unroll 1
-        for (int ch = 0; !STATES && ch < chunks; ++ch) {
             if (!wait_warp(kPvDone, ch)) break;
             fence_after();
-            const Info& f = infos[ch & 3];
-            int n_i, run_i;
-            count(f, row, &n_i, &run_i);
-            const bool ok = f.valid[warp & 3] >> lane & 1u, from_x = run_i == 0;
+            const bool ok = f.valid[place] >> lane & 1u, from_x = run_i == 0;
             const float carry = pw_hi[max(n_i - r.shift, 0)] * r.s_carry;
             const int t = first_token(ch) + row;
             T* po = const_cast<T*>(static_cast<const T*>(r.o.p)) + obase + (long long)t * r.o.st + c0;
 #pragma unroll 1
-            for (int j0 = 0; j0 < kCols; j0 += 16) {
+            for (int j0 = 32 * half; j0 < 32 * half + 32; j0 += 16) {
                 float x[16], y[16];
                 tm_ld16(x, tm_lane + kTmOi + j0);
                 tm_ld16(y, tm_lane + kTmOa + j0);
                 tm_wait_ld(x);
                 tm_wait_ld(y);
-                if (j0 + 16 == kCols) {
+                if (j0 & 16) {
                     fence_before();
                     mbar_arrive(bar(kOFree, ch));
                 }
@@ -536,18 +529,21 @@ const int eb = r.out_f32 ? 4 : 2;
         if (warp == 20 && lane == 0) {
             const int steps = (r.da + 15) / 16;
             const uint32_t q0 = base + L::kQ, k0 = base + L::kK, v0 = base + L::kV, w0 = base + L::kW, x0 = base + L::kX;
-    #pragma unroll 1
-        for (int ch = 0; ch < chunks; ++ch) {
-                const uint32_t q = q0 + (ch % NS) * L::kPanels * kPanel, k = k0 + (ch % NS) * L::kPanels * kPanel, v = v0 + (ch & 1) * kPanel;
-                if (!wait(kFull, ch)) break;
+            auto products_of_keys = [&](int ch) {  // P of a chunk
+                if (!wait(kFull, ch)) return false;
                 fence_after();
-                if (!STATES) {
-                    const uint64_t dq = desc_k(q), dk = desc_k(k);
+                const uint64_t dq = desc_k(q0 + (ch % NS) * L::kPanels * kPanel), dk = desc_k(k0 + (ch % NS) * L::kPanels * kPanel);
+                const uint32_t d = tm + kTmP + (ch & 1) * 128;
 #pragma unroll
-                    for (int s = 0; s < ROWS / 16; ++s)
-                        if (s < steps) mma_ss(tm + kTmP, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dk, (s >> 2) * kPanel + (s & 3) * 32), idesc(128, false, false), s > 0);
-                    commit(bar(kPRaw, ch));
-                }
+                for (int s = 0; s < ROWS / 16; ++s)
+                    if (s < steps) mma_ss(d, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dk, (s >> 2) * kPanel + (s & 3) * 32), idesc(128, false, false), s > 0);
+                commit(bar(kPRaw, ch));
+                return true;
+            };
+            bool going = STATES || chunks == 0 || products_of_keys(0);
+#pragma unroll 1
+            for (int ch = 0; going && ch < chunks; ++ch) {
+                const uint32_t q = q0 + (ch % NS) * L::kPanels * kPanel, k = k0 + (ch % NS) * L::kPanels * kPanel, v = v0 + (ch & 1) * kPanel;
                 if (!wait(kVwRdy, ch) || (ch > 0 && !wait(kKvFree, ch - 1))) break;
                 fence_after();
 #pragma unroll 1
@@ -557,7 +553,7 @@ const int eb = r.out_f32 ? 4 : 2;
 #pragma unroll 1
                     for (int p = 2; p >= 0; --p) {
 #pragma unroll
-                        for (int s = 0; s < kC / 16; ++s) mma_ss(tm + (tile ? kTmKV2 : kTmKV), at(dk, s * 2048), at(dw, s * 2048), idesc(64, true, true), p < 2 || s > 0);
+                        for (int s = 0; s < kC / 16; ++s) mma_ss(tm + (tile ? kTmKV2 : kTmKV), at(dk, s * 2048), at(dw, s * 2048), idesc(kCols, true, true), p < 2 || s > 0);
                         dw -= kPanel >> 4;
                     }
                 }
@@ -568,13 +564,18 @@ const int eb = r.out_f32 ? 4 : 2;
                     const uint64_t dq = desc_k(q), dx = desc_mn(x0), dv = desc_mn(v);
 #pragma unroll
                     for (int s = 0; s < ROWS / 16; ++s)
-                        if (s < steps) mma_ss(tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(64, false, true), s > 0);
+                        if (s < steps) mma_ss(tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(kCols, false, true), s > 0);
                     commit(bar(kQxDone, ch));
+                    // the next chunk's products fill the time that this one's decays take (with one buffer of q and k its tokens
+                    // come too late for that)
+                    if (NS == 2 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
                     if (!wait(kPRdy, ch)) break;
                     fence_after();
 #pragma unroll
-                    for (int s = 0; s < kC / 16; ++s) mma_ts(tm + kTmOa, tm + kTmPb + 8 * s, at(dv, s * 2048), idesc(64, false, true), s > 0);
+                    for (int s = 0; s < kC / 16; ++s)
+                        mma_ts(tm + kTmOa, tm + kTmP + (ch & 1) * 128 + operand_column(s >> 1) + 8 * (s & 1), at(dv, s * 2048), idesc(kCols, false, true), s > 0);
                     commit(bar(kPvDone, ch));
+                    if (NS == 1 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
                 }
             }
         }

@@ -200,13 +200,13 @@ int plan_launch(const Launch& l, int dtype, int kernel, int wanted) {
     int n = wanted;
     if (n == 0) {
         // Time in units of a chunk: waves of CTAs, each of them its chunks and a start-up of one and a half; a split adds
-        // the pass over keys and values that finds the parts' states (half a chunk's work) and the join.
+        // the pass over keys and values that finds the parts' states (0.4 of a chunk's work) and the join.
         const long long slots = (long long)ctas_per_sm(l, kind) * sm_count();
         double best = 0;
-        for (int m = 1; m <= std::min(kMaxSegments, std::max(1, l.c.seqlen / 256)); ++m) {
+        for (int m = 1; m <= std::min(kMaxSegments, std::max(1, chunks)); ++m) {
             const double per = (chunks + m - 1) / m;
             double t = (double)((ctas * m + slots - 1) / slots) * (per + 1.5);
-            if (m > 1) t += (double)((ctas * (m - 1) + slots - 1) / slots) * (0.5 * per + 1.5) + 1.5;
+            if (m > 1) t += (double)((ctas * (m - 1) + slots - 1) / slots) * (0.4 * per + 1.5) + 1.5;
             if (m == 1 || t < best) best = t, n = m;
         }
     }

@@ -59,7 +59,7 @@ constexpr unsigned kSpin = 1u << 22;  // polls of 64 ns and more
 constexpr uint32_t kTmP = 0, kTmOi = 256, kTmOa = 320, kTmKV = 384, kTmKV2 = 448, kTmCols = 512;
 __host__ __device__ constexpr uint32_t operand_column(int blk) { return (blk >> 1) * 64 + (blk & 1) * 16; }  // of 32 keys
 
-enum Bar { kTma, kFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
+enum Bar { kTma, kTmaV, kFull, kVFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
 
 struct Info {  // of a chunk's tokens, bit i of word i / 32 for token i; a ring of four
     unsigned valid[4], start[4];
@@ -104,18 +104,28 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) { return desc(addr, k
 __host__ __device__ constexpr uint32_t idesc(int n, bool a_mn, bool b_mn) {  // bf16 x bf16 -> fp32, 128 rows
     return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(128 / 16) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t i, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-                 "l"(b), "r"(i), "r"((uint32_t)add)
-                 : "memory");
+// Called by a whole warp, with one lane that issues: descriptors then come from the warp's uniform registers, without a
+// move from a lane's registers for every operand (a thread of its own took twice as long to issue a product).
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t i, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-                 "l"(b), "r"(i), "r"((uint32_t)add)
-                 : "memory");
+__device__ __forceinline__ void mma_ss(bool leader, uint32_t d, uint64_t a, uint64_t b, uint32_t i, bool add) {
+    if (leader)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                     "l"(b), "r"(i), "r"((uint32_t)add)
+                     : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void mma_ts(bool leader, uint32_t d, uint32_t a, uint64_t b, uint32_t i, bool add) {
+    if (leader)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                     "l"(b), "r"(i), "r"((uint32_t)add)
+                     : "memory");
+}
+// after the products that the same lane has issued
+__device__ __forceinline__ void commit(bool leader, uint32_t bar) {
+    if (leader) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -182,6 +192,10 @@ __device__ __forceinline__ bool poll(uint32_t addr, uint32_t parity, volatile ui
     return false;
 }
 
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+
 // ROWS: state rows the kernel is built for (128 or 160).  REV: tokens run from the last to the first; a constant, because
 // the hot code of all parts together has to stay in the SM's instruction cache.
 template <int ROWS, bool STATES, bool REV>
@@ -197,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     float* pw_lo = pw_hi + kPow;
     float* add = reinterpret_cast<float*>(sm + L::kAdd);
     Info* infos = reinterpret_cast<Info*>(sm + L::kInfo);
-    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4] chunks asked for
+    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4-5] chunks asked for
     volatile uint32_t* dead = misc + 1;
 
     const Run& r = l.run[blockIdx.z];
@@ -220,6 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     const int chunks = (t_end - t_begin + kC - 1) / kC;
     auto first_token = [&](int ch) { return rev ? c.seqlen - t_begin - (ch + 1) * kC : t_begin + ch * kC; };
 
+    // the weighted values of a chunk; where no queries are needed their buffers hold those of every other chunk
+    auto weighted = [&](int ch) { return STATES && (ch & 1) ? L::kQ : L::kW; };
     auto bar = [&](int kind, int chunk) { return base + L::kBar + 8 * (2 * kind + (chunk & 1)); };
     // Waits until the event of `kind` that belongs to `chunk` has happened.  Each kind has two barriers, for even and odd
     // chunks: nobody who waits is ever two chunks behind, so a phase cannot be missed.
@@ -236,12 +252,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         pw_lo[n] = (isfinite(hi) && lo == lo) ? (float)lo : 0.f;
         if (n < 32) block[rev ? n : 31 - n] = hi, pw_hi[n - 32] = 0.f;
     }
-    for (int i = tid; i < L::kBlock / 16; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+    // panels of k that the head does not reach are read as rows of the state all the same; every other byte is written first
+    for (int p = (r.da + 63) / 64; p < L::kPanels; ++p)
+        for (int i = tid; i < NS * kPanel / 16; i += kThreads)
+            *reinterpret_cast<uint4*>(sm + L::kK + (i / (kPanel / 16) * L::kPanels + p) * kPanel + i % (kPanel / 16) * 16) = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
-        misc[1] = misc[4] = 0;
+        misc[1] = misc[4] = misc[5] = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(kTma, i), 1);
+            mbar_init(bar(kTmaV, i), 1);
             mbar_init(bar(kFull, i), c.mask != nullptr ? 32 : 1);
+            mbar_init(bar(kVFull, i), c.mask != nullptr ? 32 : 1);
             mbar_init(bar(kPRaw, i), 1);
             mbar_init(bar(kPRdy, i), 256);
             mbar_init(bar(kVwRdy, i), kWeighers);
@@ -485,7 +506,8 @@ const int eb = r.out_f32 ? 4 : 2;
         const int me = tid - 256;
 #pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
-            const bool ok = wait(kFull, ch) && (ch == 0 || wait(kKvDone, ch - 1));
+            constexpr int kBack = STATES ? 2 : 1;  // buffers
+            const bool ok = wait(kVFull, ch) && (ch < kBack || wait(kKvDone, ch - kBack));
             if (!all_of(1, kWeighers, ok)) break;  // the weights of the chunk before are no longer read
             const Info& f = infos[ch & 3];
             if (me < kC) {
@@ -495,7 +517,7 @@ const int eb = r.out_f32 ? 4 : 2;
             }
             asm volatile("bar.sync 1, %0;" ::"n"(kWeighers) : "memory");
             const unsigned char* v = sm + L::kV + (ch & 1) * kPanel;
-            unsigned char* w = sm + L::kW;
+            unsigned char* w = sm + weighted(ch);
             const int at = ((me & 7) ^ (me >> 3 & 7)) << 4;  // rows 32 apart have the same swizzle
 #pragma unroll 2
             for (int i = 0; i < kC * 8 / kWeighers; ++i) {
@@ -526,55 +548,56 @@ const int eb = r.out_f32 ? 4 : 2;
     } else {
         many_registers();  // the same instruction for the four warps of the group
         // ------------------------------------------------------------------------------ products
-        if (warp == 20 && lane == 0) {
+        if (warp == 20) {
+            const bool leader = elect_lane();
             const int steps = (r.da + 15) / 16;
-            const uint32_t q0 = base + L::kQ, k0 = base + L::kK, v0 = base + L::kV, w0 = base + L::kW, x0 = base + L::kX;
+            const uint32_t q0 = base + L::kQ, k0 = base + L::kK, v0 = base + L::kV, x0 = base + L::kX;
             auto products_of_keys = [&](int ch) {  // P of a chunk
-                if (!wait(kFull, ch)) return false;
+                if (!wait_warp(kFull, ch)) return false;
                 fence_after();
                 const uint64_t dq = desc_k(q0 + (ch % NS) * L::kPanels * kPanel), dk = desc_k(k0 + (ch % NS) * L::kPanels * kPanel);
                 const uint32_t d = tm + kTmP + (ch & 1) * 128;
 #pragma unroll
                 for (int s = 0; s < ROWS / 16; ++s)
-                    if (s < steps) mma_ss(d, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dk, (s >> 2) * kPanel + (s & 3) * 32), idesc(128, false, false), s > 0);
-                commit(bar(kPRaw, ch));
+                    if (s < steps) mma_ss(leader, d, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dk, (s >> 2) * kPanel + (s & 3) * 32), idesc(128, false, false), s > 0);
+                commit(leader, bar(kPRaw, ch));
                 return true;
             };
             bool going = STATES || chunks == 0 || products_of_keys(0);
 #pragma unroll 1
             for (int ch = 0; going && ch < chunks; ++ch) {
                 const uint32_t q = q0 + (ch % NS) * L::kPanels * kPanel, k = k0 + (ch % NS) * L::kPanels * kPanel, v = v0 + (ch & 1) * kPanel;
-                if (!wait(kVwRdy, ch) || (ch > 0 && !wait(kKvFree, ch - 1))) break;
+                if ((STATES && !wait_warp(kFull, ch)) || !wait_warp(kVwRdy, ch) || (ch > 0 && !wait_warp(kKvFree, ch - 1))) break;
                 fence_after();
 #pragma unroll 1
                 for (int tile = 0; tile < (kSecond ? 2 : 1); ++tile) {  // rows 0-127; 64-191, of which 128-159 are used
                     const uint64_t dk = desc_mn(k + tile * kPanel);
-                    uint64_t dw = desc_mn(w0 + 2 * kPanel);
+                    uint64_t dw = desc_mn(base + weighted(ch) + 2 * kPanel);
 #pragma unroll 1
                     for (int p = 2; p >= 0; --p) {
 #pragma unroll
-                        for (int s = 0; s < kC / 16; ++s) mma_ss(tm + (tile ? kTmKV2 : kTmKV), at(dk, s * 2048), at(dw, s * 2048), idesc(kCols, true, true), p < 2 || s > 0);
+                        for (int s = 0; s < kC / 16; ++s) mma_ss(leader, tm + (tile ? kTmKV2 : kTmKV), at(dk, s * 2048), at(dw, s * 2048), idesc(kCols, true, true), p < 2 || s > 0);
                         dw -= kPanel >> 4;
                     }
                 }
-                commit(bar(kKvDone, ch));
+                commit(leader, bar(kKvDone, ch));
                 if (!STATES) {
-                    if (!wait(kXRdy, ch) || (ch > 0 && !wait(kOFree, ch - 1))) break;
+                    if (!wait_warp(kXRdy, ch) || (ch > 0 && !wait_warp(kOFree, ch - 1))) break;
                     fence_after();
                     const uint64_t dq = desc_k(q), dx = desc_mn(x0), dv = desc_mn(v);
 #pragma unroll
                     for (int s = 0; s < ROWS / 16; ++s)
-                        if (s < steps) mma_ss(tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(kCols, false, true), s > 0);
-                    commit(bar(kQxDone, ch));
+                        if (s < steps) mma_ss(leader, tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(kCols, false, true), s > 0);
+                    commit(leader, bar(kQxDone, ch));
                     // the next chunk's products fill the time that this one's decays take (with one buffer of q and k its tokens
                     // come too late for that)
                     if (NS == 2 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
-                    if (!wait(kPRdy, ch)) break;
+                    if (!wait_warp(kPRdy, ch)) break;
                     fence_after();
 #pragma unroll
                     for (int s = 0; s < kC / 16; ++s)
-                        mma_ts(tm + kTmOa, tm + kTmP + (ch & 1) * 128 + operand_column(s >> 1) + 8 * (s & 1), at(dv, s * 2048), idesc(kCols, false, true), s > 0);
-                    commit(bar(kPvDone, ch));
+                        mma_ts(leader, tm + kTmOa, tm + kTmP + (ch & 1) * 128 + operand_column(s >> 1) + 8 * (s & 1), at(dv, s * 2048), idesc(kCols, false, true), s > 0);
+                    commit(leader, bar(kPvDone, ch));
                     if (NS == 1 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
                 }
             }
@@ -609,41 +632,58 @@ const int eb = r.out_f32 ? 4 : 2;
                 n += __popc(vb);
                 run += __popc(sb);
             }
-            // the buffers are free
-            bool ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
-            ok = ok && (ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2))));
-            if (!__all_sync(0xffffffffu, ok)) break;
             if (lane == 0) {
                 f->n_all = n;
                 f->run_all = run;
-                const uint32_t done = bar(c.mask != nullptr ? kTma : kFull, ch);
-                tma::mbar_arrive_expect_tx(done, ((STATES ? 1 : 2) * panels + 1) * kPanel);
+            }
+            // values have two buffers, queries and keys as many as fit: each is asked for as soon as its own is free
+            const bool hand_over = c.mask != nullptr;  // by way of the warp that clears rows
+            bool ok = ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2)));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (lane == 0) {
+                const uint32_t done = bar(hand_over ? kTmaV : kVFull, ch);
+                tma::mbar_arrive_expect_tx(done, kPanel);
+                tma_load_4d(base + L::kV + (ch & 1) * kPanel, &m.v, c0, t0, head_v, b, done);
+                misc[4] = ch + 1;
+            }
+            ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (lane == 0) {
+                const uint32_t done = bar(hand_over ? kTma : kFull, ch);
+                tma::mbar_arrive_expect_tx(done, (STATES ? 1 : 2) * panels * kPanel);
                 for (int p = 0; p < panels; ++p) {
                     tma_load_4d(base + L::kK + ((ch % NS) * L::kPanels + p) * kPanel, &m.k, p * 64, t0, head_k, b, done);
                     if (!STATES) tma_load_4d(base + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel, &m.a, p * 64, t0, head_a, b, done);
                 }
-                tma_load_4d(base + L::kV + (ch & 1) * kPanel, &m.v, c0, t0, head_v, b, done);
-                misc[4] = ch + 1;
+                misc[5] = ch + 1;
+                if (NS == 1 && ch + 1 < chunks) {  // with one buffer the next chunk's would come from HBM too late
+                    for (int p = 0; p < panels; ++p) {
+                        tma_prefetch_4d(&m.k, p * 64, first_token(ch + 1), head_k, b);
+                        if (!STATES) tma_prefetch_4d(&m.a, p * 64, first_token(ch + 1), head_a, b);
+                    }
+                }
             }
             __syncwarp();
         }
 #pragma unroll 1
         for (int ch = 0; warp == 23 && c.mask != nullptr && ch < chunks; ++ch) {
-            if (!wait_warp(kTma, ch)) break;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
             const Info& f = infos[ch & 3];
-            if (f.n_all < kC) {
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
-                    if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
-                    const int at = row * 128 + (lane & 7) * 16;
-                    for (int p = 0; p < panels; ++p) {
-                        *reinterpret_cast<uint4*>(sm + L::kK + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
-                        if (!STATES) *reinterpret_cast<uint4*>(sm + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
-                    }
-                    *reinterpret_cast<uint4*>(sm + L::kV + (ch & 1) * kPanel + at) = zero;
+            if (!wait_warp(kTmaV, ch)) break;
+            for (int row = lane >> 3; row < kC && f.n_all < kC; row += 4)  // eight lanes to a row
+                if (!(f.valid[row >> 5] >> (row & 31) & 1u)) *reinterpret_cast<uint4*>(sm + L::kV + (ch & 1) * kPanel + row * 128 + (lane & 7) * 16) = zero;
+            fence_async_smem();
+            mbar_arrive(bar(kVFull, ch));
+            if (!wait_warp(kTma, ch)) break;
+            for (int row = lane >> 3; row < kC && f.n_all < kC; row += 4) {
+                if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
+                const int at = row * 128 + (lane & 7) * 16;
+                for (int p = 0; p < panels; ++p) {
+                    *reinterpret_cast<uint4*>(sm + L::kK + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
+                    if (!STATES) *reinterpret_cast<uint4*>(sm + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
                 }
-                fence_async_smem();
             }
+            fence_async_smem();
             mbar_arrive(bar(kFull, ch));
         }
     }
@@ -658,11 +698,13 @@ const int eb = r.out_f32 ? 4 : 2;
             const uint32_t last = base + L::kMisc + 8;
             mbar_init(last, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            commit(last);
+            commit(true, last);
             for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
-            const int issued = misc[4];
-            for (int ch = max(0, issued - 2); ch < issued; ++ch)
-                for (unsigned i = 0; i < kSpin && !mbar_test(bar(c.mask != nullptr ? kTma : kFull, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+            for (int kind = 0; kind < 2; ++kind) {
+                const int issued = misc[4 + kind], bars = c.mask != nullptr ? (kind ? kTma : kTmaV) : (kind ? kFull : kVFull);
+                for (int ch = max(0, issued - 2); ch < issued; ++ch)
+                    for (unsigned i = 0; i < kSpin && !mbar_test(bar(bars, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+            }
         }
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(kTmCols));

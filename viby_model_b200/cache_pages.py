@@ -30,31 +30,38 @@ class PageTable:
         self.states = list(states)
         self.device = self.states[0].device if self.states else None
         self.pages = int(self.states[0].shape[0]) if self.states and self.states[0].dim() else 0
-        n = len(self.states)
-        self._table = (_cabi.PageTensor * max(n, 1))()
-        for i, t in enumerate(self.states):
-            if t.dim() < 1:
-                raise ValueError("a state needs a first dimension: its pages")
-            if t.device.type != "cuda":
-                raise ValueError(f"state {i} must be on a CUDA device, got {t.device}")
-            if t.device != self.device:
-                raise ValueError(f"state {i} is on {t.device}, the first on {self.device}")
-            if t.shape[0] != self.pages:
-                raise ValueError(f"state {i} has {t.shape[0]} pages, the first {self.pages}")
-            if t.requires_grad and torch.is_grad_enabled():
-                raise ValueError(f"state {i} requires grad: pages are moved in place")
-            item, inner = t.element_size(), 1
-            for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-                if size > 1 and stride != inner:
-                    raise ValueError(f"state {i}: a page must be contiguous, got strides {t.stride()}")
-                inner *= size
-            if self.pages > 1 and t.stride(0) < inner:
-                raise ValueError(f"state {i}: pages overlap (stride {t.stride(0)} for {inner} values)")
-            e = self._table[i]
-            e.base, e.page_bytes = t.data_ptr(), inner * item
-            e.stride_bytes = t.stride(0) * item if self.pages > 1 else inner * item
+        n, index, pages = len(self.states), self.device.index if self.states else None, max(self.pages, 1)
+        no_grad = not torch.is_grad_enabled()
+        rows = []  # address, bytes of a page, bytes from page to page
+        for t in self.states:
+            if t.is_contiguous() and t.get_device() == index and t.dim() and t.shape[0] == self.pages and (no_grad or not t.requires_grad):
+                size = t.nbytes // pages
+                rows += (t.data_ptr(), size, size)
+            else:
+                rows += self._strided(t)
+        self._table = (C.c_int64 * max(3 * n, 1))(*rows)
         if self.pages > _cabi.PAGES_MAX_PAGES:
             raise ValueError(f"at most {_cabi.PAGES_MAX_PAGES} pages, got {self.pages}")
+
+    def _strided(self, t: torch.Tensor):
+        if t.dim() < 1:
+            raise ValueError("a state needs a first dimension: its pages")
+        if t.device.type != "cuda":
+            raise ValueError(f"a state must be on a CUDA device, got {t.device}")
+        if t.device != self.device:
+            raise ValueError(f"a state is on {t.device}, the first on {self.device}")
+        if t.shape[0] != self.pages:
+            raise ValueError(f"a state has {t.shape[0]} pages, the first {self.pages}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a state requires grad: pages are moved in place")
+        item, inner = t.element_size(), 1
+        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if size > 1 and stride != inner:
+                raise ValueError(f"a page must be contiguous, got strides {t.stride()}")
+            inner *= size
+        if self.pages > 1 and t.stride(0) < inner:
+            raise ValueError(f"pages overlap: stride {t.stride(0)} for {inner} values")
+        return t.data_ptr(), inner * item, (t.stride(0) if self.pages > 1 else inner) * item
 
     def _run(self, op: int, source=None, dst=None, n: int = 0, live=None, new_index=None, count=None) -> None:
         a = _cabi.PagesArgs()
@@ -67,7 +74,7 @@ class PageTable:
         if index is not None:
             a.index_dtype = _INDEX_DTYPES[index.dtype]
         stream = _stream_handle(self.device)
-        base, size, total = C.addressof(self._table), C.sizeof(_cabi.PageTensor), len(self.states)
+        base, size, total = C.addressof(self._table), C.sizeof(_cabi.PageTensor), len(self.states)  # three int64 each
         other = self.device.index != torch.cuda.current_device()
         if other:
             prev = torch.cuda.current_device()
@@ -82,6 +89,7 @@ class PageTable:
         finally:
             if other:
                 torch.cuda.set_device(prev)
+        torch.autograd.graph.increment_version(self.states)  # a graph that saved one of them refuses to run
 
     def _index(self, t: torch.Tensor, what: str) -> torch.Tensor:
         if not isinstance(t, torch.Tensor) or t.dim() != 1:

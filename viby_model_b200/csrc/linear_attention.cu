@@ -47,21 +47,35 @@ __global__ void __launch_bounds__(256) k_linear_join(const __grid_constant__ Lau
     }
 }
 
-// Gradients of shared heads: out[b, t, g, d] = sum over the heads of group g of part[b, t, h, d], in order of h.
+// Gradients of shared heads: out[b, t, g, d] = sum over the heads of group g of part[b, t, h, d], in order of h.  A thread
+// has four channels of one (b, t, g); bound by reading the partial sums once.
 template <int DT>
 __global__ void __launch_bounds__(256) k_linear_sum_heads(const float* part, Rows out, int heads, int seqlen, int dim, long long n) {
     using T = typename Elem<DT>::type;
-    const int groups = heads / out.group;
+    const int groups = heads / out.group, quads = (dim + 3) / 4;
+    const bool whole = dim % 4 == 0;  // rows of partial sums are 16-byte aligned
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const int d = (int)(i % dim);
-        long long rest = i / dim;
+        const int d = (int)(i % quads) * 4;
+        long long rest = i / quads;
         const int g = (int)(rest % groups);
         rest /= groups;
         const long long t = rest % seqlen, b = rest / seqlen;
         const float* p = part + ((b * seqlen + t) * heads + (long long)g * out.group) * dim + d;
-        float x = 0.f;
-        for (int j = 0; j < out.group; ++j) x += p[(long long)j * dim];
-        static_cast<T*>(const_cast<void*>(out.p))[b * out.sb + t * out.st + g * out.sh + d * out.sd] = Elem<DT>::from_float(x);
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < out.group; ++j, p += dim) {
+            if (whole) {
+                const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
+                x[0] += v.x, x[1] += v.y, x[2] += v.z, x[3] += v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < dim) x[e] += p[e];
+            }
+        }
+        T* o = static_cast<T*>(const_cast<void*>(out.p)) + b * out.sb + t * out.st + g * out.sh + d * out.sd;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < dim) o[e * out.sd] = Elem<DT>::from_float(x[e]);
     }
 }
 
@@ -224,7 +238,7 @@ cudaError_t launch_one(const Launch& l, int dtype, Kind kind, bool states_only, 
 // Enqueues the runs of `l`, split along time if the workspace allows it.
 cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, long long ws_bytes, cudaStream_t s) {
     Kind kind = pick(l, dtype, kernel);
-    for (int i = 0; i < l.runs; ++i) l.run[i].out_vec = !l.run[i].out_f32 && vector_rows(l.run[i].o, elem_bytes(dtype));
+    for (int i = 0; i < l.runs; ++i) l.run[i].out_vec = vector_rows(l.run[i].o, l.run[i].out_f32 ? 4 : elem_bytes(dtype));
     if (segments > 1 && (ws == nullptr || ws_bytes < split_bytes(l, segments))) segments = 1;
     const int chunks = (l.c.seqlen + chunk_of(kind) - 1) / chunk_of(kind);
     l.c.segments = segments;
@@ -358,7 +372,7 @@ long long part_bytes(const vc1d_linear_args& f, int heads_x, int dim) {
 }
 
 cudaError_t sum_heads(int dtype, const float* part, const Rows& out, const vc1d_linear_args& f, int dim, cudaStream_t s) {
-    const long long n = (long long)f.batch * f.seqlen * (f.heads / out.group) * dim;
+    const long long n = (long long)f.batch * f.seqlen * (f.heads / out.group) * ((dim + 3) / 4);
     const int grid = (int)std::min<long long>((n + 255) / 256, 32LL * sm_count());
     note_launch("linear_sum_heads");
     switch (dtype) {

@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, DAP == 256 ? 1 : 2) k_linear_mma(con
             const int t0 = t_begin + chunk * kChunk + grp * 16;
             const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
             __syncwarp();  // every lane has read its fragments of q
-            if (r.out_vec) {
+            if (r.out_vec && !r.out_f32) {
 #pragma unroll
                 for (int n = 0; n < kN; n += 2)
                     stsm4(aq + 2 * (n * 8), Hf::pack(O[n][0], O[n][1]), Hf::pack(O[n][2], O[n][3]), Hf::pack(O[n + 1][0], O[n + 1][1]),

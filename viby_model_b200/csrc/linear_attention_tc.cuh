@@ -59,7 +59,7 @@ constexpr unsigned kSpin = 1u << 22;  // polls of 64 ns and more
 constexpr uint32_t kTmP = 0, kTmOi = 256, kTmOa = 320, kTmKV = 384, kTmKV2 = 448, kTmCols = 512;
 __host__ __device__ constexpr uint32_t operand_column(int blk) { return (blk >> 1) * 64 + (blk & 1) * 16; }  // of 32 keys
 
-enum Bar { kTma, kTmaV, kFull, kVFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
+enum Bar { kTmaQ, kTmaK, kTmaV, kQFull, kKFull, kVFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
 
 struct Info {  // of a chunk's tokens, bit i of word i / 32 for token i; a ring of four
     unsigned valid[4], start[4];
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     float* pw_lo = pw_hi + kPow;
     float* add = reinterpret_cast<float*>(sm + L::kAdd);
     Info* infos = reinterpret_cast<Info*>(sm + L::kInfo);
-    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4-5] chunks asked for
+    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4-6] chunks asked for
     volatile uint32_t* dead = misc + 1;
 
     const Run& r = l.run[blockIdx.z];
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     // reaches past the first token
     const int t_begin = seg * c.seg_chunks * kC;
     const int t_end = min(c.seqlen, t_begin + c.seg_chunks * kC);
-    const int chunks = (t_end - t_begin + kC - 1) / kC;
-    auto first_token = [&](int ch) { return rev ? c.seqlen - t_begin - (ch + 1) * kC : t_begin + ch * kC; };
+    int chunks = (t_end - t_begin + kC - 1) / kC, skipped = 0;  // padding at either end is not walked
+    auto first_token = [&](int ch) { return rev ? c.seqlen - t_begin - (skipped + ch + 1) * kC : t_begin + (skipped + ch) * kC; };
 
     // the weighted values of a chunk; where no queries are needed their buffers hold those of every other chunk
     auto weighted = [&](int ch) { return STATES && (ch & 1) ? L::kQ : L::kW; };
@@ -257,12 +257,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         for (int i = tid; i < NS * kPanel / 16; i += kThreads)
             *reinterpret_cast<uint4*>(sm + L::kK + (i / (kPanel / 16) * L::kPanels + p) * kPanel + i % (kPanel / 16) * 16) = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
-        misc[1] = misc[4] = misc[5] = 0;
+        misc[1] = misc[4] = misc[5] = misc[6] = 0;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(kTma, i), 1);
-            mbar_init(bar(kTmaV, i), 1);
-            mbar_init(bar(kFull, i), c.mask != nullptr ? 32 : 1);
-            mbar_init(bar(kVFull, i), c.mask != nullptr ? 32 : 1);
+            for (int x = 0; x < 3; ++x) {
+                mbar_init(bar(kTmaQ + x, i), 1);
+                mbar_init(bar(kQFull + x, i), c.mask != nullptr ? 32 : 1);
+            }
             mbar_init(bar(kPRaw, i), 1);
             mbar_init(bar(kPRdy, i), 256);
             mbar_init(bar(kVwRdy, i), kWeighers);
@@ -284,6 +284,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     __syncthreads();
     fence_after();
     const uint32_t tm = misc[0];
+    if (c.mask != nullptr && chunks > 0) {
+        // chunks between the first and the last valid token, in the run's order; the outputs of the others are zeros
+        int* range = reinterpret_cast<int*>(add);
+        if (tid == 0) range[0] = chunks, range[1] = -1;
+        __syncthreads();
+        int lo = chunks, hi = -1;
+        for (int i = t_begin + tid; i < t_end; i += kThreads)
+            if (mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + (long long)(rev ? c.seqlen - 1 - i : i) * c.mask_st)) {
+                const int ch = (i - t_begin) / kC;
+                lo = min(lo, ch);
+                hi = max(hi, ch);
+            }
+        if (hi >= 0) {
+            atomicMin(&range[0], lo);
+            atomicMax(&range[1], hi);
+        }
+        __syncthreads();
+        lo = range[0], hi = range[1];
+        __syncthreads();  // the array gets its own use
+        if (!STATES) {
+            const int eb = r.out_f32 ? 4 : 2, before = max(0, min(t_end, t_begin + lo * kC) - t_begin), after = hi < 0 ? t_end : min(t_end, t_begin + (hi + 1) * kC);
+            char* o = const_cast<char*>(static_cast<const char*>(r.o.p)) + ((long long)b * r.o.sb + (long long)h * r.o.sh + (long long)c0 * r.o.sd) * eb;
+            for (int i = tid; i < (before + t_end - after) * kCols; i += kThreads) {
+                const int row = i / kCols, col = i % kCols, at = row < before ? t_begin + row : after + row - before;
+                if (col >= cols) continue;
+                char* q = o + ((long long)(rev ? c.seqlen - 1 - at : at) * r.o.st + col * r.o.sd) * eb;
+                if (r.out_f32)
+                    *reinterpret_cast<float*>(q) = 0.f;
+                else
+                    *reinterpret_cast<T*>(q) = __float2bfloat16_rn(0.f);
+            }
+        }
+        skipped = hi < 0 ? 0 : lo;
+        chunks = hi < 0 ? 0 : hi - lo + 1;
+    }
     const uint32_t tm_lane = tm + ((uint32_t)(warp & 3) << 21);  // a warp reaches the 32 lanes of its place in its group
 
     // Valid tokens and sequence starts of a chunk up to and with token i, in the run's order.
@@ -332,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         bool fine = true;
 #pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
-            if (!wait_warp(kFull, ch) || !wait_warp(kKvDone, ch)) {
+            if (!wait_warp(kKFull, ch) || !wait_warp(kKvDone, ch)) {
                 fine = false;
                 break;
             }
@@ -392,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
 #pragma unroll 1
         for (int ch = 0; !STATES && ch < chunks; ++ch) {
-            if (!wait_warp(kFull, ch) || !wait_warp(kPRaw, ch)) break;
+            if (!wait_warp(kQFull, ch) || !wait_warp(kPRaw, ch)) break;
             fence_after();
             const uint32_t tm_p = tm_lane + kTmP + (ch & 1) * 128;
             const Info& f = infos[ch & 3];
@@ -474,7 +509,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                     x[j] = ok ? o : 0.f;
                 }
                 if (t >= 0 && t < c.seqlen) {
-                    if (r.out_vec) {
+                    if (r.out_vec && r.out_f32) {
+                        float* q = reinterpret_cast<float*>(const_cast<void*>(r.o.p)) + obase + (long long)t * r.o.st + c0 + j0;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            if (j0 + 4 * u < cols) *reinterpret_cast<float4*>(q + 4 * u) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+                    } else if (r.out_vec) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
                             if (j0 + 8 * u < cols)
@@ -553,7 +593,7 @@ const int eb = r.out_f32 ? 4 : 2;
             const int steps = (r.da + 15) / 16;
             const uint32_t q0 = base + L::kQ, k0 = base + L::kK, v0 = base + L::kV, x0 = base + L::kX;
             auto products_of_keys = [&](int ch) {  // P of a chunk
-                if (!wait_warp(kFull, ch)) return false;
+                if (!wait_warp(kKFull, ch) || !wait_warp(kQFull, ch)) return false;
                 fence_after();
                 const uint64_t dq = desc_k(q0 + (ch % NS) * L::kPanels * kPanel), dk = desc_k(k0 + (ch % NS) * L::kPanels * kPanel);
                 const uint32_t d = tm + kTmP + (ch & 1) * 128;
@@ -563,11 +603,11 @@ const int eb = r.out_f32 ? 4 : 2;
                 commit(leader, bar(kPRaw, ch));
                 return true;
             };
-            bool going = STATES || chunks == 0 || products_of_keys(0);
+            bool going = STATES || NS == 1 || chunks == 0 || products_of_keys(0);
 #pragma unroll 1
             for (int ch = 0; going && ch < chunks; ++ch) {
                 const uint32_t q = q0 + (ch % NS) * L::kPanels * kPanel, k = k0 + (ch % NS) * L::kPanels * kPanel, v = v0 + (ch & 1) * kPanel;
-                if ((STATES && !wait_warp(kFull, ch)) || !wait_warp(kVwRdy, ch) || (ch > 0 && !wait_warp(kKvFree, ch - 1))) break;
+                if (!wait_warp(kKFull, ch) || !wait_warp(kVwRdy, ch) || (ch > 0 && !wait_warp(kKvFree, ch - 1))) break;
                 fence_after();
 #pragma unroll 1
                 for (int tile = 0; tile < (kSecond ? 2 : 1); ++tile) {  // rows 0-127; 64-191, of which 128-159 are used
@@ -582,6 +622,8 @@ const int eb = r.out_f32 ? 4 : 2;
                 }
                 commit(leader, bar(kKvDone, ch));
                 if (!STATES) {
+                    // with one buffer of keys the state's products go first: theirs is the longer way to the next chunk
+                    if (NS == 1 && !products_of_keys(ch)) break;
                     if (!wait_warp(kXRdy, ch) || (ch > 0 && !wait_warp(kOFree, ch - 1))) break;
                     fence_after();
                     const uint64_t dq = desc_k(q), dx = desc_mn(x0), dv = desc_mn(v);
@@ -589,8 +631,7 @@ const int eb = r.out_f32 ? 4 : 2;
                     for (int s = 0; s < ROWS / 16; ++s)
                         if (s < steps) mma_ss(leader, tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(kCols, false, true), s > 0);
                     commit(leader, bar(kQxDone, ch));
-                    // the next chunk's products fill the time that this one's decays take (with one buffer of q and k its tokens
-                    // come too late for that)
+                    // the next chunk's products fill the time that this one's decays take
                     if (NS == 2 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
                     if (!wait_warp(kPRdy, ch)) break;
                     fence_after();
@@ -598,7 +639,6 @@ const int eb = r.out_f32 ? 4 : 2;
                     for (int s = 0; s < kC / 16; ++s)
                         mma_ts(leader, tm + kTmOa, tm + kTmP + (ch & 1) * 128 + operand_column(s >> 1) + 8 * (s & 1), at(dv, s * 2048), idesc(kCols, false, true), s > 0);
                     commit(leader, bar(kPvDone, ch));
-                    if (NS == 1 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
                 }
             }
         }
@@ -636,55 +676,55 @@ const int eb = r.out_f32 ? 4 : 2;
                 f->n_all = n;
                 f->run_all = run;
             }
-            // values have two buffers, queries and keys as many as fit: each is asked for as soon as its own is free
-            const bool hand_over = c.mask != nullptr;  // by way of the warp that clears rows
+            // values have two buffers, keys and queries as many as fit: each is asked for as soon as its own is free
+            const int hand_over = c.mask != nullptr ? kTmaQ : kQFull;  // by way of the warp that clears rows
+            auto ask = [&](const CUtensorMap* map, int what, int panel0, int c_first, int head, uint32_t to) {
+                if (lane == 0) {
+                    const uint32_t done = bar(hand_over + what, ch);
+                    tma::mbar_arrive_expect_tx(done, panel0 * kPanel);
+                    for (int p = 0; p < panel0; ++p) tma_load_4d(base + to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
+                    misc[4 + what] = ch + 1;
+                }
+            };
             bool ok = ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2)));
             if (!__all_sync(0xffffffffu, ok)) break;
-            if (lane == 0) {
-                const uint32_t done = bar(hand_over ? kTmaV : kVFull, ch);
-                tma::mbar_arrive_expect_tx(done, kPanel);
-                tma_load_4d(base + L::kV + (ch & 1) * kPanel, &m.v, c0, t0, head_v, b, done);
-                misc[4] = ch + 1;
-            }
-            ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kQxDone, ch - NS)));
+            ask(&m.v, 2, 1, c0, head_v, L::kV + (ch & 1) * kPanel);
+            ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kPRaw, ch - NS)));
             if (!__all_sync(0xffffffffu, ok)) break;
-            if (lane == 0) {
-                const uint32_t done = bar(hand_over ? kTma : kFull, ch);
-                tma::mbar_arrive_expect_tx(done, (STATES ? 1 : 2) * panels * kPanel);
+            ask(&m.k, 1, panels, 0, head_k, L::kK + (ch % NS) * L::kPanels * kPanel);
+            if (!STATES) {
+                ok = ch < NS || wait(kQxDone, ch - NS);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                ask(&m.a, 0, panels, 0, head_a, L::kQ + (ch % NS) * L::kPanels * kPanel);
+            }
+            if (NS == 1 && ch + 1 < chunks && lane == 0) {  // with one buffer the next chunk's would come from HBM too late
                 for (int p = 0; p < panels; ++p) {
-                    tma_load_4d(base + L::kK + ((ch % NS) * L::kPanels + p) * kPanel, &m.k, p * 64, t0, head_k, b, done);
-                    if (!STATES) tma_load_4d(base + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel, &m.a, p * 64, t0, head_a, b, done);
-                }
-                misc[5] = ch + 1;
-                if (NS == 1 && ch + 1 < chunks) {  // with one buffer the next chunk's would come from HBM too late
-                    for (int p = 0; p < panels; ++p) {
-                        tma_prefetch_4d(&m.k, p * 64, first_token(ch + 1), head_k, b);
-                        if (!STATES) tma_prefetch_4d(&m.a, p * 64, first_token(ch + 1), head_a, b);
-                    }
+                    tma_prefetch_4d(&m.k, p * 64, first_token(ch + 1), head_k, b);
+                    if (!STATES) tma_prefetch_4d(&m.a, p * 64, first_token(ch + 1), head_a, b);
                 }
             }
             __syncwarp();
         }
 #pragma unroll 1
         for (int ch = 0; warp == 23 && c.mask != nullptr && ch < chunks; ++ch) {
-            const uint4 zero = make_uint4(0, 0, 0, 0);
             const Info& f = infos[ch & 3];
-            if (!wait_warp(kTmaV, ch)) break;
-            for (int row = lane >> 3; row < kC && f.n_all < kC; row += 4)  // eight lanes to a row
-                if (!(f.valid[row >> 5] >> (row & 31) & 1u)) *reinterpret_cast<uint4*>(sm + L::kV + (ch & 1) * kPanel + row * 128 + (lane & 7) * 16) = zero;
-            fence_async_smem();
-            mbar_arrive(bar(kVFull, ch));
-            if (!wait_warp(kTma, ch)) break;
-            for (int row = lane >> 3; row < kC && f.n_all < kC; row += 4) {
-                if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
-                const int at = row * 128 + (lane & 7) * 16;
-                for (int p = 0; p < panels; ++p) {
-                    *reinterpret_cast<uint4*>(sm + L::kK + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
-                    if (!STATES) *reinterpret_cast<uint4*>(sm + L::kQ + ((ch % NS) * L::kPanels + p) * kPanel + at) = zero;
+            bool ok = true;
+#pragma unroll 1
+            for (int what = 2; what >= (STATES ? 1 : 0); --what) {  // values, keys, queries: in the order they are asked for
+                ok = wait_warp(kTmaQ + what, ch);
+                if (!ok) break;
+                if (f.n_all < kC) {
+                    unsigned char* to = sm + (what == 2 ? L::kV + (ch & 1) * kPanel : (what == 1 ? L::kK : L::kQ) + (ch % NS) * L::kPanels * kPanel);
+                    for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
+                        if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
+                        for (int p = 0; p < (what == 2 ? 1 : panels); ++p)
+                            *reinterpret_cast<uint4*>(to + p * kPanel + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async_smem();
                 }
+                mbar_arrive(bar(kQFull + what, ch));
             }
-            fence_async_smem();
-            mbar_arrive(bar(kFull, ch));
+            if (!ok) break;
         }
     }
     __syncwarp();
@@ -700,10 +740,10 @@ const int eb = r.out_f32 ? 4 : 2;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             commit(true, last);
             for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
-            for (int kind = 0; kind < 2; ++kind) {
-                const int issued = misc[4 + kind], bars = c.mask != nullptr ? (kind ? kTma : kTmaV) : (kind ? kFull : kVFull);
-                for (int ch = max(0, issued - 2); ch < issued; ++ch)
-                    for (unsigned i = 0; i < kSpin && !mbar_test(bar(bars, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+            for (int what = 0; what < 3; ++what) {
+                const int asked = misc[4 + what], kind = (c.mask != nullptr ? kTmaQ : kQFull) + what;
+                for (int ch = max(0, asked - 2); ch < asked; ++ch)
+                    for (unsigned i = 0; i < kSpin && !mbar_test(bar(kind, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
             }
         }
         __syncwarp();

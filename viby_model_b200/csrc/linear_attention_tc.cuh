@@ -192,10 +192,6 @@ __device__ __forceinline__ bool poll(uint32_t addr, uint32_t parity, volatile ui
     return false;
 }
 
-__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
-    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
-}
-
 // ROWS: state rows the kernel is built for (128 or 160).  REV: tokens run from the last to the first; a constant, because
 // the hot code of all parts together has to stay in the SM's instruction cache.
 template <int ROWS, bool STATES, bool REV>
@@ -263,10 +259,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 mbar_init(bar(kTmaQ + x, i), 1);
                 mbar_init(bar(kQFull + x, i), c.mask != nullptr ? 32 : 1);
             }
-            mbar_init(bar(kPRaw, i), 1);
+            mbar_init(bar(kPRaw, i), 2);   // the products, and the chunk's info
             mbar_init(bar(kPRdy, i), 256);
             mbar_init(bar(kVwRdy, i), kWeighers);
-            mbar_init(bar(kKvDone, i), 1);
+            mbar_init(bar(kKvDone, i), 2);
             mbar_init(bar(kKvFree, i), kSecond ? 160 : 128);
             mbar_init(bar(kXRdy, i), kSecond ? 160 : 128);
             mbar_init(bar(kQxDone, i), 1);
@@ -367,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         bool fine = true;
 #pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
-            if (!wait_warp(kKFull, ch) || !wait_warp(kKvDone, ch)) {
+            if (!wait_warp(kKvDone, ch)) {
                 fine = false;
                 break;
             }
@@ -427,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         const long long obase = (long long)b * r.o.sb + (long long)h * r.o.sh;
 #pragma unroll 1
         for (int ch = 0; !STATES && ch < chunks; ++ch) {
-            if (!wait_warp(kQFull, ch) || !wait_warp(kPRaw, ch)) break;
+            if (!wait_warp(kPRaw, ch)) break;
             fence_after();
             const uint32_t tm_p = tm_lane + kTmP + (ch & 1) * 128;
             const Info& f = infos[ch & 3];
@@ -646,6 +642,7 @@ const int eb = r.out_f32 ? 4 : 2;
         // ------------------------------------------------------------------------------ tokens
         const Maps& m = maps.run[blockIdx.z];
         const int panels = (r.da + 63) / 64;
+        const bool leader = elect_lane();
         const int head_a = h / r.a.group, head_k = h / r.k.group, head_v = h / r.v.group;
 #pragma unroll 1
         for (int ch = 0; warp == 21 && ch < chunks; ++ch) {
@@ -676,33 +673,40 @@ const int eb = r.out_f32 ? 4 : 2;
                 f->n_all = n;
                 f->run_all = run;
             }
-            // values have two buffers, keys and queries as many as fit: each is asked for as soon as its own is free
+            __syncwarp();
             const int hand_over = c.mask != nullptr ? kTmaQ : kQFull;  // by way of the warp that clears rows
-            auto ask = [&](const CUtensorMap* map, int what, int panel0, int c_first, int head, uint32_t to) {
-                if (lane == 0) {
-                    const uint32_t done = bar(hand_over + what, ch);
-                    tma::mbar_arrive_expect_tx(done, panel0 * kPanel);
-                    for (int p = 0; p < panel0; ++p) tma_load_4d(base + to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
+            auto ask = [&](const CUtensorMap* map, int what, int n_panels, int c_first, int head, uint32_t to) {
+                const uint32_t done = bar(hand_over + what, ch);
+                if (leader) {
+                    tma::mbar_arrive_expect_tx(done, n_panels * kPanel);
                     misc[4 + what] = ch + 1;
                 }
+                for (int p = 0; p < n_panels; ++p)
+                    if (leader) tma_load_4d(base + to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
             };
-            bool ok = ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPvDone, ch - 2)));
-            if (!__all_sync(0xffffffffu, ok)) break;
-            ask(&m.v, 2, 1, c0, head_v, L::kV + (ch & 1) * kPanel);
-            ok = ch < NS || (wait(kKvDone, ch - NS) && (STATES || wait(kPRaw, ch - NS)));
-            if (!__all_sync(0xffffffffu, ok)) break;
+            auto all = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
+            auto ask_values = [&]() {
+                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) return false;
+                ask(&m.v, 2, 1, c0, head_v, L::kV + (ch & 1) * kPanel);
+                return true;
+            };
+            // Values have two buffers, keys and queries as many as fit.  Each is asked for when its own is free: with two of
+            // each, keys first; with one, values, because the next chunk's wait for nothing else.
+            if (!all(ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPRaw, ch - 2))))) break;
+            if (leader) {  // the info is there for those who wait for the products
+                if (!STATES) mbar_arrive(bar(kPRaw, ch));
+                mbar_arrive(bar(kKvDone, ch));
+            }
+            if (NS == 1) {
+                if (!ask_values()) break;
+                if (!all(ch < 1 || (wait(kKvDone, ch - 1) && (STATES || wait(kPRaw, ch - 1))))) break;
+            }
             ask(&m.k, 1, panels, 0, head_k, L::kK + (ch % NS) * L::kPanels * kPanel);
             if (!STATES) {
-                ok = ch < NS || wait(kQxDone, ch - NS);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (!all(ch < NS || wait(kQxDone, ch - NS))) break;
                 ask(&m.a, 0, panels, 0, head_a, L::kQ + (ch % NS) * L::kPanels * kPanel);
             }
-            if (NS == 1 && ch + 1 < chunks && lane == 0) {  // with one buffer the next chunk's would come from HBM too late
-                for (int p = 0; p < panels; ++p) {
-                    tma_prefetch_4d(&m.k, p * 64, first_token(ch + 1), head_k, b);
-                    if (!STATES) tma_prefetch_4d(&m.a, p * 64, first_token(ch + 1), head_a, b);
-                }
-            }
+            if (NS == 2 && !ask_values()) break;
             __syncwarp();
         }
 #pragma unroll 1
@@ -710,7 +714,8 @@ const int eb = r.out_f32 ? 4 : 2;
             const Info& f = infos[ch & 3];
             bool ok = true;
 #pragma unroll 1
-            for (int what = 2; what >= (STATES ? 1 : 0); --what) {  // values, keys, queries: in the order they are asked for
+            for (int turn = 0; turn < (STATES ? 2 : 3); ++turn) {  // in the order they are asked for
+                const int what = NS == 1 ? 2 - turn : (STATES ? 1 + turn : (turn + 1) % 3);  // 2: values, 1: keys, 0: queries
                 ok = wait_warp(kTmaQ + what, ch);
                 if (!ok) break;
                 if (f.n_all < kC) {

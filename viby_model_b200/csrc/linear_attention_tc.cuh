@@ -16,7 +16,8 @@
 //     warps 16-19  the same for the keys 64-127 and the columns 32-63
 //     warp 20      issues the products
 //     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
-//     warp 23      where there is a mask: clears the rows of masked tokens, whatever they hold, and hands the chunk over
+//     warp 23      says which tokens of a chunk count; where there is a mask, clears the rows of masked ones, whatever they
+//                  hold, and hands the chunk over
 // The parts are short programs of a few hundred instructions at five or so cycles each, so it is the longest part that
 // sets the pace: that is why there are so many, and twice the warps for the weighted values.
 // While one chunk's P is being decayed, the next chunk's tokens arrive and the state runs ahead.
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         for (int i = 0; i < 2; ++i) {
             for (int x = 0; x < 3; ++x) {
                 mbar_init(bar(kTmaQ + x, i), 1);
-                mbar_init(bar(kQFull + x, i), c.mask != nullptr ? 32 : 1);
+                mbar_init(bar(kQFull + x, i), c.mask != nullptr ? 32 : kQFull + x == kVFull ? 2 : 1);  // values: and the info
             }
             mbar_init(bar(kPRaw, i), 2);   // the products, and the chunk's info
             mbar_init(bar(kPRdy, i), 256);
@@ -647,6 +648,42 @@ const int eb = r.out_f32 ? 4 : 2;
 #pragma unroll 1
         for (int ch = 0; warp == 21 && ch < chunks; ++ch) {
             const int t0 = first_token(ch);
+            const int hand_over = c.mask != nullptr ? kTmaQ : kQFull;  // by way of the warp that clears rows
+            auto ask = [&](const CUtensorMap* map, int what, int n_panels, int c_first, int head, uint32_t to) {
+                const uint32_t done = bar(hand_over + what, ch);
+                if (leader) {
+                    tma::mbar_arrive_expect_tx(done, n_panels * kPanel);
+                    misc[4 + what] = ch + 1;
+                }
+                for (int p = 0; p < n_panels; ++p)
+                    if (leader) tma_load_4d(base + to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
+            };
+            auto all = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
+            auto ask_values = [&]() {
+                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) return false;
+                ask(&m.v, 2, 1, c0, head_v, L::kV + (ch & 1) * kPanel);
+                return true;
+            };
+            // Values have two buffers, keys and queries as many as fit.  Each is asked for when its own is free: with two of
+            // each, keys first; with one, values, because the next chunk's wait for nothing else.
+            if (!all(ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPRaw, ch - 2))))) break;
+            if (NS == 1) {
+                if (!ask_values()) break;
+                if (!all(ch < 1 || (wait(kKvDone, ch - 1) && (STATES || wait(kPRaw, ch - 1))))) break;
+            }
+            ask(&m.k, 1, panels, 0, head_k, L::kK + (ch % NS) * L::kPanels * kPanel);
+            if (!STATES) {
+                if (!all(ch < NS || wait(kQxDone, ch - NS))) break;
+                ask(&m.a, 0, panels, 0, head_a, L::kQ + (ch % NS) * L::kPanels * kPanel);
+            }
+            if (NS == 2 && !ask_values()) break;
+            __syncwarp();
+        }
+#pragma unroll 1
+        for (int ch = 0; warp == 23 && ch < chunks; ++ch) {
+            // nobody looks at the chunk before the last but one any more
+            if (ch >= 2 && !(wait_warp(kKvFree, ch - 2) && (STATES || wait_warp(kPvDone, ch - 2)))) break;
+            const int t0 = first_token(ch);
             // the tokens of the chunk that count, and the sequence starts in the run's order
             Info* f = infos + (ch & 3);
             int n = 0, run = 0;
@@ -674,54 +711,22 @@ const int eb = r.out_f32 ? 4 : 2;
                 f->run_all = run;
             }
             __syncwarp();
-            const int hand_over = c.mask != nullptr ? kTmaQ : kQFull;  // by way of the warp that clears rows
-            auto ask = [&](const CUtensorMap* map, int what, int n_panels, int c_first, int head, uint32_t to) {
-                const uint32_t done = bar(hand_over + what, ch);
-                if (leader) {
-                    tma::mbar_arrive_expect_tx(done, n_panels * kPanel);
-                    misc[4 + what] = ch + 1;
-                }
-                for (int p = 0; p < n_panels; ++p)
-                    if (leader) tma_load_4d(base + to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
-            };
-            auto all = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
-            auto ask_values = [&]() {
-                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) return false;
-                ask(&m.v, 2, 1, c0, head_v, L::kV + (ch & 1) * kPanel);
-                return true;
-            };
-            // Values have two buffers, keys and queries as many as fit.  Each is asked for when its own is free: with two of
-            // each, keys first; with one, values, because the next chunk's wait for nothing else.
-            if (!all(ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPRaw, ch - 2))))) break;
-            if (leader) {  // the info is there for those who wait for the products
+            if (leader) {  // for those who wait for the products or the values
                 if (!STATES) mbar_arrive(bar(kPRaw, ch));
                 mbar_arrive(bar(kKvDone, ch));
+                if (c.mask == nullptr) mbar_arrive(bar(kVFull, ch));
             }
-            if (NS == 1) {
-                if (!ask_values()) break;
-                if (!all(ch < 1 || (wait(kKvDone, ch - 1) && (STATES || wait(kPRaw, ch - 1))))) break;
-            }
-            ask(&m.k, 1, panels, 0, head_k, L::kK + (ch % NS) * L::kPanels * kPanel);
-            if (!STATES) {
-                if (!all(ch < NS || wait(kQxDone, ch - NS))) break;
-                ask(&m.a, 0, panels, 0, head_a, L::kQ + (ch % NS) * L::kPanels * kPanel);
-            }
-            if (NS == 2 && !ask_values()) break;
-            __syncwarp();
-        }
-#pragma unroll 1
-        for (int ch = 0; warp == 23 && c.mask != nullptr && ch < chunks; ++ch) {
-            const Info& f = infos[ch & 3];
+            if (c.mask == nullptr) continue;
             bool ok = true;
 #pragma unroll 1
             for (int turn = 0; turn < (STATES ? 2 : 3); ++turn) {  // in the order they are asked for
                 const int what = NS == 1 ? 2 - turn : (STATES ? 1 + turn : (turn + 1) % 3);  // 2: values, 1: keys, 0: queries
                 ok = wait_warp(kTmaQ + what, ch);
                 if (!ok) break;
-                if (f.n_all < kC) {
+                if (f->n_all < kC) {
                     unsigned char* to = sm + (what == 2 ? L::kV + (ch & 1) * kPanel : (what == 1 ? L::kK : L::kQ) + (ch % NS) * L::kPanels * kPanel);
                     for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
-                        if (f.valid[row >> 5] >> (row & 31) & 1u) continue;
+                        if (f->valid[row >> 5] >> (row & 31) & 1u) continue;
                         for (int p = 0; p < (what == 2 ? 1 : panels); ++p)
                             *reinterpret_cast<uint4*>(to + p * kPanel + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }

@@ -34,7 +34,7 @@ class PageTable:
         no_grad = not torch.is_grad_enabled()
         rows = []  # address, bytes of a page, bytes from page to page
         for t in self.states:
-            if t.is_contiguous() and t.get_device() == index and t.dim() and t.shape[0] == self.pages and (no_grad or not t.requires_grad):
+            if t.get_device() == index and t.is_contiguous() and t.dim() and t.size(0) == self.pages and (no_grad or not t.requires_grad):
                 size = t.nbytes // pages
                 rows += (t.data_ptr(), size, size)
             else:

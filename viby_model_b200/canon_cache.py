@@ -9,13 +9,18 @@ device (eval_model.py:41-54).
 
 The states this package's kernels update are plain ``[batch, dim, state_len]`` tensors, changed in place, so all
 of that is index and attribute work on the host; these helpers do it for any object that allows attributes (a
-``Cache``, a ``types.SimpleNamespace``).  They hold no state of their own and launch nothing themselves.
+``Cache``, a ``types.SimpleNamespace``).  They hold no state of their own.  ``reorder(..., inplace=True)``, ``fork``,
+``free`` and ``compact`` move the rows of every state in place with one kernel launch (``cache_pages``): a row of all
+states together is the page of one request or beam.  Other state tensors that belong to the same requests, such as linear
+attention states, move along when given as ``also``.
 """
 from __future__ import annotations
 
 from typing import Iterable, Iterator, Optional, Tuple
 
 import torch
+
+from .cache_pages import PageTable
 
 CANON_POSITIONS = ("a", "b", "c", "d")
 _PREFIX = "canon_cache_"
@@ -60,10 +65,43 @@ def _canon_lists(cache) -> Iterator[Tuple[str, list]]:
             yield name, value
 
 
-def reorder(cache, beam_idx: torch.Tensor):
+def page_table(cache, also: Iterable[torch.Tensor] = ()) -> PageTable:
+    """The pages (rows) of every Canon state and seqlens vector of the cache and of the tensors in ``also``.  A tensor that
+    is held at several places counts once.  CUDA tensors with one number of rows; see ``cache_pages.PageTable``."""
+    entries = {id(t): t for _, slots in _canon_lists(cache) for t in slots if t is not None} if cache is not None else {}
+    entries.update((id(t), t) for t in also)
+    return PageTable(entries.values())
+
+
+def fork(cache, src: torch.Tensor, dst: torch.Tensor, also: Iterable[torch.Tensor] = ()):
+    """Row ``dst[i]`` of every state takes over row ``src[i]``, in place: a request is copied, or forked into several
+    samples by naming it several times.  Returns the cache."""
+    page_table(cache, also).copy(src, dst)
+    return cache
+
+
+def free(cache, rows: torch.Tensor, also: Iterable[torch.Tensor] = ()):
+    """Clears the given rows of every state to zero, as a new request finds them, in place.  Returns the cache."""
+    page_table(cache, also).free(rows)
+    return cache
+
+
+def compact(cache, live: torch.Tensor, also: Iterable[torch.Tensor] = ()) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Moves the rows of live requests (``live[rows]``, bool) to the front of every state, in place, so that decode steps
+    run on ``state[:n]``.  Returns ``(new_index, count)`` on the device: where each row is afterwards, and n."""
+    return page_table(cache, also).compact(live)
+
+
+def reorder(cache, beam_idx: torch.Tensor, *, inplace: bool = False, also: Iterable[torch.Tensor] = ()):
     """Beam search: row ``i`` of every Canon state (and of every seqlens vector) becomes row ``beam_idx[i]``
-    (model/model.py:1340-1364).  The entries are replaced by new tensors, as ``index_select`` makes them;
-    the key/value part of the cache is the cache's own business (``cache.reorder_cache``).  Returns the cache."""
+    (model/model.py:1340-1364).  The entries are replaced by new tensors, as ``index_select`` makes them; with
+    ``inplace`` they keep their memory and one launch reorders them all, and the tensors in ``also`` with them.
+    The key/value part of the cache is the cache's own business (``cache.reorder_cache``).  Returns the cache."""
+    if inplace:
+        page_table(cache, also).reorder(beam_idx)
+        return cache
+    if list(also):
+        raise ValueError("also= needs inplace=True")
     if cache is None:
         return None
     for _, slots in _canon_lists(cache):

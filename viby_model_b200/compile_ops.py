@@ -1,6 +1,6 @@
 """torch.library registration of the operators, so that ``torch.compile(fullgraph=True)`` (how the
 reference compiles its model for evaluation, eval_model.py:157) can trace a model that calls
-``causal_conv1d_fn`` / ``causal_conv1d_update``: each becomes one opaque node of the graph, with a
+``causal_conv1d_fn`` / ``causal_conv1d_update`` / ``linear_attention_fn`` / ``linear_attention_update``: each becomes one opaque node of the graph, with a
 shape function (``register_fake``) and a backward formula (``register_autograd``).
 
 The eager entry points keep calling the C ABI directly (a decode step is launch-bound and the
@@ -13,6 +13,7 @@ from typing import Optional, Tuple
 
 import torch
 
+from . import linear_attention as la
 from . import ops
 
 _ACT = {0: None, 1: "silu"}
@@ -143,3 +144,64 @@ def _(x, conv_state, weight, bias, dy, cache_seqlens, activation, residual):
 
 
 torch.library.register_autograd("vc1d::update_fn", _update_backward, setup_context=_update_setup)
+
+
+@torch.library.custom_op("vc1d::linear_attention", mutates_args=(), device_types="cuda")
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, seq_idx: Optional[torch.Tensor],
+                     initial_states: Optional[torch.Tensor], mask: Optional[torch.Tensor], scale: float,
+                     want_state: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """o (and, with want_state, the final state) of linear_attention_fn."""
+    o, state = la._forward(q, k, v, log_decay, seq_idx, initial_states, want_state, None, mask, scale, None, None, 0)
+    return o, state if state is not None else q.new_empty(0, dtype=torch.float32)
+
+
+@linear_attention.register_fake
+def _(q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state):
+    o = q.new_empty((q.shape[0], q.shape[1], q.shape[2], v.shape[3]))
+    shape = (q.shape[0], q.shape[2], q.shape[3], v.shape[3]) if want_state else (0,)
+    return o, q.new_empty(shape, dtype=torch.float32)
+
+
+@torch.library.custom_op("vc1d::linear_attention_bwd", mutates_args=(), device_types="cuda")
+def linear_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, dout: torch.Tensor,
+                         seq_idx: Optional[torch.Tensor], initial_states: Optional[torch.Tensor],
+                         dfinal_states: Optional[torch.Tensor], mask: Optional[torch.Tensor], scale: float
+                         ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    dq, dk, dv, dinit = la.linear_attention_bwd(q, k, v, log_decay, dout, seq_idx, initial_states, dfinal_states,
+                                                attention_mask=mask, scale=scale)
+    return dq, dk, dv, dinit if dinit is not None else q.new_empty(0, dtype=torch.float32)
+
+
+@linear_attention_bwd.register_fake
+def _(q, k, v, log_decay, dout, seq_idx, initial_states, dfinal_states, mask, scale):
+    dinit = q.new_empty(initial_states.shape if initial_states is not None else (0,), dtype=torch.float32)
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), dinit
+
+
+def _linear_setup(ctx, inputs, output):
+    q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state = inputs
+    ctx.save_for_backward(q, k, v, log_decay, seq_idx, initial_states, mask)
+    ctx.scale = scale
+    ctx.want_state = want_state
+
+
+def _linear_backward(ctx, dout, dstate):
+    q, k, v, log_decay, seq_idx, init, mask = ctx.saved_tensors
+    dq, dk, dv, dinit = torch.ops.vc1d.linear_attention_bwd(q, k, v, log_decay, dout, seq_idx, init,
+                                                            dstate if ctx.want_state else None, mask, ctx.scale)
+    return dq, dk, dv, None, None, dinit if init is not None else None, None, None, None
+
+
+torch.library.register_autograd("vc1d::linear_attention", _linear_backward, setup_context=_linear_setup)
+
+
+@torch.library.custom_op("vc1d::linear_attention_update", mutates_args=("state",), device_types="cuda")
+def linear_attention_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: torch.Tensor, log_decay: torch.Tensor,
+                            mask: Optional[torch.Tensor], scale: float) -> torch.Tensor:
+    """o of linear_attention_update; state is updated in place.  Forward only."""
+    return la._update(q, k, v, state, log_decay, mask, scale, None)
+
+
+@linear_attention_update.register_fake
+def _(q, k, v, state, log_decay, mask, scale):
+    return q.new_empty((q.shape[0], q.shape[1], v.shape[2]))

@@ -158,3 +158,13 @@ def test_another_stream():
         V.reorder_pages(states, idx)
     s.synchronize()
     same(states, want)
+
+
+def test_pages_far_apart():
+    far = (1 << 32) + 48  # bytes from page to page
+    buf = torch.zeros(3 * far, dtype=torch.uint8, device=DEV)
+    t = buf.as_strided((3, 4096), (far, 1))
+    t.copy_(torch.randint(0, 255, (3, 4096)).to(torch.uint8))
+    want = O.move_pages([t], [2, 0, 1])
+    V.reorder_pages([t], torch.tensor([2, 0, 1], device=DEV))
+    same([t], want)

@@ -482,3 +482,52 @@ def test_results_repeat_bit_for_bit():
     first = V.linear_attention_bwd(q, k, v, g, do, None, s0, ds)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, V.linear_attention_bwd(q, k, v, g, do, None, s0, ds)))
+
+
+@pytest.mark.parametrize("dtype,kernel", [("bf16", "tc"), ("bf16", "mma"), ("f16", "mma"), ("f32", "simt")])
+@pytest.mark.parametrize("which", ["right", "left", "holes"])
+def test_long_masked_rows(dtype, kernel, which):
+    """Many chunks: whole chunks of padding at either end, rows without a token, holes."""
+    T = 900
+    t = torch.arange(T)[None]
+    lens = torch.tensor([[900], [517], [128], [0]])
+    m = {"right": t < lens, "left": t >= T - lens, "holes": (t // 131) % 2 == torch.tensor([[0], [1], [0], [1]])}[which]
+    backward_case(DTYPES[dtype], 4, T, 2, 1, 2, 64, 48, mask=m, init=True, final=True, poison=float("nan"), kernel=kernel)
+    forward_case(DTYPES[dtype], 4, T, 2, 1, 2, 64, 48, mask=m, init=True, final=True, poison=float("nan"), kernel=kernel)
+    forward_case(DTYPES[dtype], 4, T, 2, 1, 2, 64, 48, mask=m, init=True, final=True, kernel=kernel, segments=3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_past_32_bits(dtype):
+    """Tokens far apart in memory: the last lies more than 2^32 elements behind the first."""
+    dt = DTYPES[dtype]
+    T, H, D, far = 300, 1, 32, 1 << 24
+    q, k, v, do, *_ = make(1, T, H, H, H, D, D, dt)
+    buf = torch.empty(T * far, dtype=dt, device=DEV).view(1, T, far)
+    views = [buf[:, :, i * D: (i + 1) * D].unflatten(-1, (H, D)) for i in range(4)]
+    for x, y in zip(views, (q, k, v)):
+        x.copy_(y)
+    out = torch.empty(T * far, dtype=dt, device=DEV).view(1, T, far)[:, :, :D].unflatten(-1, (H, D))
+    g = decays(H)
+    V.linear_attention_fn(*views[:3], dev(g), out=out)
+    ref, _ = O.linear_attention(q, k, v, g)
+    M, _ = magnitudes(q, k, v, g)
+    check(out, ref, tolerance(ref, M, dt, D, T, dt != torch.float32), "out")
+
+
+def test_update_of_states_far_apart():
+    far = (1 << 31) + 64
+    pool = torch.empty(3 * far, device=DEV)
+    q, k, v, _, s0, _ = make(3, 1, 2, 2, 2, 32, 32, torch.bfloat16)
+    state = pool.as_strided((3, 2, 32, 32), (far, 1024, 32, 1))
+    state.copy_(s0)
+    g = decays(2)
+    o = V.linear_attention_update(dev(q[:, 0]), dev(k[:, 0]), dev(v[:, 0]), state, dev(g))
+    ref, ref_s = O.linear_attention(q, k, v, g, initial=s0)
+    M, M_s = magnitudes(q, k, v, g, s0)
+    check(o, ref[:, 0], tolerance(ref, M, torch.bfloat16, 32, 64, False)[:, 0], "out")
+    check(state, ref_s, tolerance(ref_s, M_s, torch.bfloat16, 32, 64, False, torch.float32), "state")
+
+
+def test_no_wait_of_a_kernel_has_run_out():
+    assert V.tma_timeouts() == 0

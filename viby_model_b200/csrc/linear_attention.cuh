@@ -174,7 +174,7 @@ inline int mma_rows(const Launch& l) {
 }
 inline int slab_of(const Launch& l, Kind k) { return k == kMma && mma_rows(l) == 160 ? 80 : 64; }
 inline int chunk_of(Kind k) { return k == kTc ? 128 : kChunk; }
-inline int ctas_per_sm(const Launch& l, Kind k) { return k == kMma && mma_rows(l) <= 160 ? 2 : 1; }
+inline int ctas_per_sm(const Launch& l, Kind k) { return (k == kMma && mma_rows(l) <= 160) || (k == kSimt && largest_rows(l) <= 96) ? 2 : 1; }
 
 }  // namespace lin
 

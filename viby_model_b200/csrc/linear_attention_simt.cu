@@ -31,12 +31,13 @@ __device__ __forceinline__ void tile_fma(float (&acc)[4][4], const float4 (&a)[4
 }
 
 template <int DT, bool STATES>
-__global__ void __launch_bounds__(kThreads) k_linear_simt(const __grid_constant__ Launch l) {
+__global__ void __launch_bounds__(kThreads, 2) k_linear_simt(const __grid_constant__ Launch l) {
     using E = Elem<DT>;
     using T = typename E::type;
     extern __shared__ __align__(16) float sm[];
     __shared__ ChunkInfo info;
     __shared__ float2 pw[kPowers];
+    __shared__ float add[kChunk];
 
     const Run& r = l.run[blockIdx.z];
     const Common& c = l.c;
@@ -81,6 +82,11 @@ __global__ void __launch_bounds__(kThreads) k_linear_simt(const __grid_constant_
     const T* pk = static_cast<const T*>(r.k.p) + (long long)b * r.k.sb + (long long)(h / r.k.group) * r.k.sh;
     const T* pv = static_cast<const T*>(r.v.p) + (long long)b * r.v.sb + (long long)(h / r.v.group) * r.v.sh;
 
+    auto wide_rows = [&](const T* p, const Rows& x, int channels) {
+        return DT == VC1D_F32 && x.sd == 1 && channels % 4 == 0 && x.st % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+    };
+    const bool wide_a = wide_rows(pa, r.a, r.da), wide_k = wide_rows(pk, r.k, r.da), wide_v = wide_rows(pv + (long long)c0 * r.v.sd, r.v, cols);
+
     const int ti = (tid / 16) * 4, tj = (tid % 16) * 4;  // this thread's 4 x 4 tile of a 64 x 64 product
     double seg_factor = 1.0;
 
@@ -88,17 +94,29 @@ __global__ void __launch_bounds__(kThreads) k_linear_simt(const __grid_constant_
         __syncthreads();  // the tiles of the chunk before are no longer read
         if (tid < 32) chunk_info(c, r.reverse, b, t0, t_end, &info);
         __syncthreads();
-        for (int i = tid; i < kChunk * dap; i += kThreads) {
-            const int row = i / dap, d = i % dap;
-            const bool ok = d < r.da && (info.valid[row >> 5] >> (row & 31) & 1u);
-            const long long t = t0 + row;
-            if (!STATES) sa[row * rs + d] = ok ? E::to_float(pa[t * r.a.st + d * r.a.sd]) : 0.f;
-            sk[row * rs + d] = ok ? E::to_float(pk[t * r.k.st + d * r.k.sd]) : 0.f;
-        }
-        for (int i = tid; i < kChunk * kSlab; i += kThreads) {
-            const int row = i / kSlab, d = i % kSlab;
-            const bool ok = d < cols && (info.valid[row >> 5] >> (row & 31) & 1u);
-            sv[i] = ok ? E::to_float(pv[(long long)(t0 + row) * r.v.st + (long long)(c0 + d) * r.v.sd]) : 0.f;
+        // a warp per row: rows of masked tokens and channels past the head's end become zeros, unread
+        auto fetch = [&](const T* src, long long st, long long sd, int channels, int padded, float* dst, int stride, bool wide) {
+#pragma unroll 2
+            for (int row = tid >> 5; row < kChunk; row += kThreads / 32) {
+                const bool ok = info.valid[row >> 5] >> (row & 31) & 1u;
+                const T* p = src + (long long)(t0 + row) * st;
+                if (wide) {  // fp32, channel stride 1, 16-byte aligned rows
+                    for (int d = (tid & 31) * 4; d < padded; d += 128) {
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (ok && d < channels) x = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + d));
+                        *reinterpret_cast<float4*>(dst + row * stride + d) = x;
+                    }
+                } else {
+                    for (int d = tid & 31; d < padded; d += 32) dst[row * stride + d] = ok && d < channels ? E::to_float(p[d * sd]) : 0.f;
+                }
+            }
+        };
+        if (!STATES) fetch(pa, r.a.st, r.a.sd, r.da, dap, sa, rs, wide_a);
+        fetch(pk, r.k.st, r.k.sd, r.da, dap, sk, rs, wide_k);
+        fetch(pv + (long long)c0 * r.v.sd, r.v.st, r.v.sd, cols, kSlab, sv, kSlab, wide_v);
+        if (tid < kChunk) {  // what a token's key weighs in the state after the chunk
+            const int code = info.code[tid];
+            add[tid] = (code >> 16) == info.run_all ? pw[info.n_all - (code & 0xffff) + r.shift].x * r.s_add : 0.f;
         }
         __syncthreads();
         const int n_all = info.n_all, run_all = info.run_all;
@@ -176,22 +194,16 @@ __global__ void __launch_bounds__(kThreads) k_linear_simt(const __grid_constant_
                 }
             }
         }
-        // the state: X' = a^{n_C} X + sum_j w_j k_j v_j^T.  k's rows take their weight first.
-        __syncthreads();
-        for (int i = tid; i < kChunk * dap; i += kThreads) {
-            const int row = i / dap, d = i % dap;
-            const int code = info.code[row];
-            const float w = (code >> 16) == run_all ? pw[n_all - (code & 0xffff) + r.shift].x * r.s_add : 0.f;
-            sk[row * rs + d] = (code >> 16) == run_all ? sk[row * rs + d] * w : 0.f;
-        }
-        __syncthreads();
+        // the state: X' = a^{n_C} X + sum_j w_j k_j v_j^T
+        __syncthreads();  // the queries have read it
         const float2 f = pw[n_all];
         for (int i0 = tid / 16 * 4; i0 < dap; i0 += kThreads / 16 * 4) {
             float acc[4][4] = {};
 #pragma unroll 4
             for (int j = 0; j < kChunk; ++j) {
                 const float4 x = ld4(sk + j * rs + i0), y = ld4(sv + j * kSlab + tj);
-                const float xs[4] = {x.x, x.y, x.z, x.w};
+                const float w = add[j];
+                const float xs[4] = {x.x * w, x.y * w, x.z * w, x.w * w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     acc[i][0] = fmaf(xs[i], y.x, acc[i][0]);

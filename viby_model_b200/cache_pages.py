@@ -11,6 +11,9 @@ Index tensors live on the device of the states.  An index outside ``0..pages-1``
 from __future__ import annotations
 
 import ctypes as C
+from array import array
+from itertools import repeat
+from operator import attrgetter
 from typing import Iterable, Tuple
 
 import torch
@@ -18,6 +21,7 @@ import torch
 from . import _cabi
 from .ops import _stream_handle
 
+_nbytes, _requires_grad = attrgetter("nbytes"), attrgetter("requires_grad")
 _INDEX_DTYPES = {torch.int32: _cabi.VC1D_I32, torch.int64: _cabi.VC1D_I64}
 
 
@@ -30,16 +34,19 @@ class PageTable:
         self.states = list(states)
         self.device = self.states[0].device if self.states else None
         self.pages = int(self.states[0].shape[0]) if self.states and self.states[0].dim() else 0
-        n, index, pages = len(self.states), self.device.index if self.states else None, max(self.pages, 1)
-        no_grad = not torch.is_grad_enabled()
-        rows = []  # address, bytes of a page, bytes from page to page
-        for t in self.states:
-            if t.get_device() == index and t.is_contiguous() and t.dim() and t.size(0) == self.pages and (no_grad or not t.requires_grad):
-                size = t.nbytes // pages
-                rows += (t.data_ptr(), size, size)
-            else:
-                rows += self._strided(t)
-        self._table = (C.c_int64 * max(3 * n, 1))(*rows)
+        # three numbers a tensor: address, bytes of a page, bytes from page to page.  A model's cache has many small
+        # states, so the common case asks each attribute of all of them at once.
+        table = array("q", bytes(24 * len(self.states)))
+        index = self.device.index if self.states else None
+        if (self.pages > 0 and all(map(torch.Tensor.is_contiguous, self.states)) and all(map(index.__eq__, map(torch.Tensor.get_device, self.states)))
+                and all(map(torch.Tensor.dim, self.states)) and all(map(self.pages.__eq__, map(torch.Tensor.size, self.states, repeat(0))))
+                and not (torch.is_grad_enabled() and any(map(_requires_grad, self.states)))):
+            table[0::3] = array("q", map(torch.Tensor.data_ptr, self.states))
+            table[1::3] = table[2::3] = array("q", map(self.pages.__rfloordiv__, map(_nbytes, self.states)))
+        else:
+            for n, t in enumerate(self.states):
+                table[3 * n: 3 * n + 3] = array("q", self._strided(t))
+        self._table = table
         if self.pages > _cabi.PAGES_MAX_PAGES:
             raise ValueError(f"at most {_cabi.PAGES_MAX_PAGES} pages, got {self.pages}")
 
@@ -74,7 +81,7 @@ class PageTable:
         if index is not None:
             a.index_dtype = _INDEX_DTYPES[index.dtype]
         stream = _stream_handle(self.device)
-        base, size, total = C.addressof(self._table), C.sizeof(_cabi.PageTensor), len(self.states)  # three int64 each
+        base, size, total = self._table.buffer_info()[0], C.sizeof(_cabi.PageTensor), len(self.states)
         other = self.device.index != torch.cuda.current_device()
         if other:
             prev = torch.cuda.current_device()

@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(256) k_linear_sum_heads(const float* part, Row
         const long long t = rest % seqlen, b = rest / seqlen;
         const float* p = part + ((b * seqlen + t) * heads + (long long)g * out.group) * dim + d;
         float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int j = 0; j < out.group; ++j, p += dim) {
             if (whole) {
                 const float4 v = __ldcs(reinterpret_cast<const float4*>(p));

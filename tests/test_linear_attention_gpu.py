@@ -529,5 +529,17 @@ def test_update_of_states_far_apart():
     check(state, ref_s, tolerance(ref_s, M_s, torch.bfloat16, 32, 64, False, torch.float32), "state")
 
 
+@pytest.mark.parametrize("dtype,kernel", [("bf16", "tc"), ("f16", "mma"), ("f32", "simt")])
+def test_whole_and_partly_masked_chunks_in_every_order(dtype, kernel):
+    """Rows whose chunks of 128 are whole, holed or empty, in many orders."""
+    T, B = 128 * 7 + 50, 24
+    g = torch.Generator().manual_seed(11)
+    kind = torch.randint(0, 3, (B, 8), generator=g).repeat_interleave(128, 1)[:, :T]  # 0 whole, 1 holed, 2 empty
+    m = (kind == 0) | ((kind == 1) & (torch.rand(B, T, generator=g) < 0.7))
+    for segments in (0, 3):
+        forward_case(DTYPES[dtype], B, T, 1, 1, 1, 32, 32, mask=m, init=True, final=True, poison=float("nan"), kernel=kernel, segments=segments)
+        backward_case(DTYPES[dtype], B, T, 1, 1, 1, 32, 32, mask=m, init=True, final=True, poison=float("nan"), kernel=kernel, segments=segments)
+
+
 def test_no_wait_of_a_kernel_has_run_out():
     assert V.tma_timeouts() == 0

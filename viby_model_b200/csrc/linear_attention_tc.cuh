@@ -48,6 +48,7 @@ constexpr int kC = 128;               // tokens of a chunk
 constexpr int kThreads = 768;
 constexpr int kSmallRegs = 64, kLargeRegs = 112;  // four groups and two: six times the 80 of the launch
 constexpr int kWeighers = 256;
+constexpr int kWholeChunks = 4096;  // chunks that are looked over beforehand; later ones count as not whole
 constexpr int kPow = kC + 2;          // a^0 .. a^(kC + 1)
 constexpr int kCols = 64;             // columns of a slab
 constexpr int kPanel = kC * 128;      // bytes of a panel of 128 rows
@@ -86,7 +87,8 @@ struct Layout {
     static constexpr int kBlock = kX + ROWS * 128;
     static constexpr int kPowers = kBlock + 256;  // 32 zeros before them
     static constexpr int kAdd = kPowers + 8 * kPow;
-    static constexpr int kInfo = kAdd + 4 * kC;
+    static constexpr int kWhole = kAdd + 4 * kC;  // bit per chunk: no token is masked
+    static constexpr int kInfo = kWhole + kWholeChunks / 8;
     static constexpr int kBar = (kInfo + 4 * (int)sizeof(Info) + 15) & ~15;
     static constexpr int kMisc = kBar + 8 * 2 * kBars;
     static constexpr int kBytes = kMisc + 32;
@@ -233,6 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
 
     // the weighted values of a chunk; where no queries are needed their buffers hold those of every other chunk
     auto weighted = [&](int ch) { return STATES && (ch & 1) ? L::kQ : L::kW; };
+    unsigned* whole = reinterpret_cast<unsigned*>(sm + L::kWhole);
+    // whether rows of the chunk may have to be cleared: the copy then reports to the warp that does so
+    auto to_clear = [&](int ch) { return c.mask != nullptr && !(skipped + ch < kWholeChunks && (whole[(skipped + ch) >> 5] >> ((skipped + ch) & 31) & 1u)); };
     auto bar = [&](int kind, int chunk) { return base + L::kBar + 8 * (2 * kind + (chunk & 1)); };
     // Waits until the event of `kind` that belongs to `chunk` has happened.  Each kind has two barriers, for even and odd
     // chunks: nobody who waits is ever two chunks behind, so a phase cannot be missed.
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         for (int i = 0; i < 2; ++i) {
             for (int x = 0; x < 3; ++x) {
                 mbar_init(bar(kTmaQ + x, i), 1);
-                mbar_init(bar(kQFull + x, i), c.mask != nullptr ? 32 : kQFull + x == kVFull ? 2 : 1);  // values: and the info
+                mbar_init(bar(kQFull + x, i), kQFull + x == kVFull ? 2 : 1);  // values: and the chunk's info
             }
             mbar_init(bar(kPRaw, i), 2);   // the products, and the chunk's info
             mbar_init(bar(kPRdy, i), 256);
@@ -285,20 +290,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         // chunks between the first and the last valid token, in the run's order; the outputs of the others are zeros
         int* range = reinterpret_cast<int*>(add);
         if (tid == 0) range[0] = chunks, range[1] = -1;
+        for (int i = tid; i < kWholeChunks / 32; i += kThreads) whole[i] = 0;
         __syncthreads();
-        int lo = chunks, hi = -1;
-        for (int i = t_begin + tid; i < t_end; i += kThreads)
-            if (mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + (long long)(rev ? c.seqlen - 1 - i : i) * c.mask_st)) {
-                const int ch = (i - t_begin) / kC;
-                lo = min(lo, ch);
-                hi = max(hi, ch);
+        for (int ch = warp; ch < chunks; ch += kThreads / 32) {
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int i = t_begin + ch * kC + 32 * w + lane;
+                const bool v = i < t_end && mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + (long long)(rev ? c.seqlen - 1 - i : i) * c.mask_st);
+                n += __popc(__ballot_sync(0xffffffffu, v));
             }
-        if (hi >= 0) {
-            atomicMin(&range[0], lo);
-            atomicMax(&range[1], hi);
+            if (lane == 0 && n > 0) {
+                atomicMin(&range[0], ch);
+                atomicMax(&range[1], ch);
+                if (n == kC && ch < kWholeChunks) atomicOr(&whole[ch >> 5], 1u << (ch & 31));
+            }
         }
         __syncthreads();
-        lo = range[0], hi = range[1];
+        const int lo = range[0], hi = range[1];
         __syncthreads();  // the array gets its own use
         if (!STATES) {
             const int eb = r.out_f32 ? 4 : 2, before = max(0, min(t_end, t_begin + lo * kC) - t_begin), after = hi < 0 ? t_end : min(t_end, t_begin + (hi + 1) * kC);
@@ -342,10 +351,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 }
             }
             const int n = src == nullptr ? 0 : cols;
+            if (step == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) {
-                X[j] = j < n ? *src : 0.f;
-                src += step;
+                for (int j = 0; j < kCols; j += 4) {
+                    const float4 x = j < n ? *reinterpret_cast<const float4*>(src + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    X[j] = x.x, X[j + 1] = x.y, X[j + 2] = x.z, X[j + 3] = x.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    X[j] = j < n ? *src : 0.f;
+                    src += step;
+                }
             }
         }
         auto store_x = [&]() {
@@ -405,10 +422,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                                 : r.xT.p + (long long)b * r.xT.sb + (long long)h * r.xT.sh + (long long)row * r.xT.sr;
             const long long sc = STATES ? 1 : r.xT.sc;
             dst += c0 * sc;
+            if (sc == 1 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) {
-                if (j < cols) *dst = X[j];
-                dst += sc;
+                for (int j = 0; j < kCols; j += 4)
+                    if (j < cols) *reinterpret_cast<float4*>(dst + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    if (j < cols) *dst = X[j];
+                    dst += sc;
+                }
             }
             if (STATES && slab == 0 && row == 0) {
                 const float hi = (float)seg_factor;
@@ -644,24 +667,35 @@ const int eb = r.out_f32 ? 4 : 2;
         const Maps& m = maps.run[blockIdx.z];
         const int panels = (r.da + 63) / 64;
         const bool leader = elect_lane();
+        if (warp == 21 && leader) {
+            tma::prefetch_tensormap(&m.k);
+            tma::prefetch_tensormap(&m.v);
+            if (!STATES) tma::prefetch_tensormap(&m.a);
+        }
         const int head_a = h / r.a.group, head_k = h / r.k.group, head_v = h / r.v.group;
 #pragma unroll 1
         for (int ch = 0; warp == 21 && ch < chunks; ++ch) {
             const int t0 = first_token(ch);
-            const int hand_over = c.mask != nullptr ? kTmaQ : kQFull;  // by way of the warp that clears rows
+            const int hand_over = to_clear(ch) ? kTmaQ : kQFull;
             auto ask = [&](const CUtensorMap* map, int what, int n_panels, int c_first, int head, uint32_t to) {
                 const uint32_t done = bar(hand_over + what, ch);
                 if (leader) {
                     tma::mbar_arrive_expect_tx(done, n_panels * kPanel);
+                    tma_load_4d(to, map, c_first, t0, head, b, done);
+                }
+#pragma unroll
+                for (int p = 1; p < L::kPanels; ++p)
+                    if (leader && p < n_panels) tma_load_4d(to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
+                if (leader) {
+                    // the other barrier goes through its phase of this chunk too: phases are counted in chunks
+                    if (hand_over == kQFull && c.mask != nullptr) mbar_arrive(bar(kTmaQ + what, ch));
                     misc[4 + what] = ch + 1;
                 }
-                for (int p = 0; p < n_panels; ++p)
-                    if (leader) tma_load_4d(base + to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
             };
             auto all = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
             auto ask_values = [&]() {
                 if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) return false;
-                ask(&m.v, 2, 1, c0, head_v, L::kV + (ch & 1) * kPanel);
+                ask(&m.v, 2, 1, c0, head_v, base + L::kV + (ch & 1) * kPanel);
                 return true;
             };
             // Values have two buffers, keys and queries as many as fit.  Each is asked for when its own is free: with two of
@@ -671,10 +705,10 @@ const int eb = r.out_f32 ? 4 : 2;
                 if (!ask_values()) break;
                 if (!all(ch < 1 || (wait(kKvDone, ch - 1) && (STATES || wait(kPRaw, ch - 1))))) break;
             }
-            ask(&m.k, 1, panels, 0, head_k, L::kK + (ch % NS) * L::kPanels * kPanel);
+            ask(&m.k, 1, panels, 0, head_k, base + L::kK + (ch % NS) * L::kPanels * kPanel);
             if (!STATES) {
                 if (!all(ch < NS || wait(kQxDone, ch - NS))) break;
-                ask(&m.a, 0, panels, 0, head_a, L::kQ + (ch % NS) * L::kPanels * kPanel);
+                ask(&m.a, 0, panels, 0, head_a, base + L::kQ + (ch % NS) * L::kPanels * kPanel);
             }
             if (NS == 2 && !ask_values()) break;
             __syncwarp();
@@ -714,16 +748,16 @@ const int eb = r.out_f32 ? 4 : 2;
             if (leader) {  // for those who wait for the products or the values
                 if (!STATES) mbar_arrive(bar(kPRaw, ch));
                 mbar_arrive(bar(kKvDone, ch));
-                if (c.mask == nullptr) mbar_arrive(bar(kVFull, ch));
+                mbar_arrive(bar(kVFull, ch));
             }
-            if (c.mask == nullptr) continue;
+            if (!to_clear(ch)) continue;
             bool ok = true;
 #pragma unroll 1
             for (int turn = 0; turn < (STATES ? 2 : 3); ++turn) {  // in the order they are asked for
                 const int what = NS == 1 ? 2 - turn : (STATES ? 1 + turn : (turn + 1) % 3);  // 2: values, 1: keys, 0: queries
                 ok = wait_warp(kTmaQ + what, ch);
                 if (!ok) break;
-                if (f->n_all < kC) {
+                {
                     unsigned char* to = sm + (what == 2 ? L::kV + (ch & 1) * kPanel : (what == 1 ? L::kK : L::kQ) + (ch % NS) * L::kPanels * kPanel);
                     for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
                         if (f->valid[row >> 5] >> (row & 31) & 1u) continue;
@@ -732,7 +766,8 @@ const int eb = r.out_f32 ? 4 : 2;
                     }
                     fence_async_smem();
                 }
-                mbar_arrive(bar(kQFull + what, ch));
+                __syncwarp();
+                if (leader) mbar_arrive(bar(kQFull + what, ch));
             }
             if (!ok) break;
         }
@@ -751,9 +786,9 @@ const int eb = r.out_f32 ? 4 : 2;
             commit(true, last);
             for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
             for (int what = 0; what < 3; ++what) {
-                const int asked = misc[4 + what], kind = (c.mask != nullptr ? kTmaQ : kQFull) + what;
+                const int asked = misc[4 + what];
                 for (int ch = max(0, asked - 2); ch < asked; ++ch)
-                    for (unsigned i = 0; i < kSpin && !mbar_test(bar(kind, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+                    for (unsigned i = 0; i < kSpin && !mbar_test(bar((to_clear(ch) ? kTmaQ : kQFull) + what, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
             }
         }
         __syncwarp();

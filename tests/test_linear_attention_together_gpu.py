@@ -229,3 +229,39 @@ def test_refusals_on_the_device():
         V.compact_pages([s0], torch.ones(2, device=DEV))
     with bad:
         V.reorder_pages([s0, idx], idx)  # the index is one of the states
+
+
+def test_a_decay_that_wants_a_gradient_is_refused_whatever_else_wants_one():
+    q, k, v, *_ = (t.to(DEV) for t in make(1, 8, 2, 2, 2, 16, 16, torch.bfloat16))
+    g = decays(2).to(DEV).requires_grad_()
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="no gradient"):
+            V.linear_attention_fn(x, k, v, g)
+    with pytest.raises(ValueError, match="no gradient"):
+        V.linear_attention_update(q[:, 0], k[:, 0], v[:, 0], torch.zeros(1, 2, 16, 16, device=DEV), g)
+    with torch.no_grad():
+        V.linear_attention_fn(q, k, v, g)
+    V.linear_attention_fn(q.clone().requires_grad_(), k, v, g.detach())
+
+
+def test_repeated_calls_with_other_data_alignment_and_devices_of_the_same_signature():
+    """A call's checked arguments are remembered by shapes and strides: data elsewhere, at odd addresses, in other
+    dtypes of the mask, has to come out the same."""
+    q, k, v, _, s0, _ = make(2, 130, 2, 2, 2, 64, 64, torch.bfloat16)
+    g = decays(2).to(DEV)
+    want = V.linear_attention_fn(q.to(DEV), k.to(DEV), v.to(DEV), g, None, s0.to(DEV), True, kernel="simt")
+    ref, ref_s = O.linear_attention(q, k, v, decays(2), initial=s0)
+    M, M_s = magnitudes(q, k, v, decays(2), s0)
+    for turn in range(4):
+        args = []
+        for x in (q, k, v):
+            buf = torch.empty(x.numel() + 8, dtype=x.dtype, device=DEV)
+            at = (0, 1, 8, 3)[turn]
+            buf[at: at + x.numel()] = x.reshape(-1).to(DEV)
+            args.append(buf[at: at + x.numel()].view(x.shape))
+        o, s = V.linear_attention_fn(*args, g, None, s0.to(DEV), True)
+        check(o, ref, tolerance(ref, M, torch.bfloat16, 64, 130, True), "out")
+        check(s, ref_s, tolerance(ref_s, M_s, torch.bfloat16, 64, 130, True, torch.float32), "state")
+        state = s0.to(DEV)
+        V.linear_attention_update(args[0][:, 0], args[1][:, 0], args[2][:, 0], state, g)
+    assert want[0].shape == o.shape

@@ -38,7 +38,7 @@ class PageTable:
         # states, so the common case asks each attribute of all of them at once.
         table = array("q", bytes(24 * len(self.states)))
         index = self.device.index if self.states else None
-        if (self.pages > 0 and all(map(torch.Tensor.is_contiguous, self.states)) and all(map(index.__eq__, map(torch.Tensor.get_device, self.states)))
+        if (self.pages > 0 and self.device.type == "cuda" and all(map(torch.Tensor.is_contiguous, self.states)) and all(map(index.__eq__, map(torch.Tensor.get_device, self.states)))
                 and all(map(torch.Tensor.dim, self.states)) and all(map(self.pages.__eq__, map(torch.Tensor.size, self.states, repeat(0))))
                 and not (torch.is_grad_enabled() and any(map(_requires_grad, self.states)))):
             table[0::3] = array("q", map(torch.Tensor.data_ptr, self.states))

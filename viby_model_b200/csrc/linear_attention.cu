@@ -118,7 +118,8 @@ int check_forward(const vc1d_linear_args* a) {
         if (!writable(n.o, a->out_strides)) return VC1D_E_STRIDE;
         const Range o = extent(a->out, eb, n.o, a->out_strides);
         if (overlap(o, extent(a->q, eb, n.q, a->q_strides)) || overlap(o, extent(a->k, eb, n.k, a->k_strides)) ||
-            overlap(o, extent(a->v, eb, n.v, a->v_strides)))
+            overlap(o, extent(a->v, eb, n.v, a->v_strides)) ||
+            (a->initial_state != nullptr && overlap(o, extent(a->initial_state, 4, n.s, a->initial_strides))))
             return VC1D_E_ALIAS;
     }
     if (a->final_state != nullptr) {
@@ -303,9 +304,16 @@ int check_backward(const vc1d_linear_bwd_args* a) {
         const Range in[4] = {extent(f.q, eb, n.q, f.q_strides), extent(f.k, eb, n.k, f.k_strides), extent(f.v, eb, n.v, f.v_strides),
                              extent(a->dout, eb, n.o, a->dout_strides)};
         const Range out[3] = {extent(a->dq, eb, n.q, a->dq_strides), extent(a->dk, eb, n.k, a->dk_strides), extent(a->dv, eb, n.v, a->dv_strides)};
-        for (const Range& o : out)
+        for (const Range& o : out) {
             for (const Range& i : in)
                 if (overlap(o, i)) return VC1D_E_ALIAS;
+            if (f.initial_state != nullptr && overlap(o, extent(f.initial_state, 4, n.s, f.initial_strides))) return VC1D_E_ALIAS;
+            if (a->dfinal != nullptr && overlap(o, extent(a->dfinal, 4, n.s, a->dfinal_strides))) return VC1D_E_ALIAS;
+            if (a->dinitial != nullptr && overlap(o, extent(a->dinitial, 4, n.s, a->dinitial_strides))) return VC1D_E_ALIAS;
+        }
+        if (a->dinitial != nullptr)
+            for (const Range& i : in)
+                if (overlap(i, extent(a->dinitial, 4, n.s, a->dinitial_strides))) return VC1D_E_ALIAS;
         if (overlap(out[0], out[1]) || overlap(out[0], out[2]) || overlap(out[1], out[2])) return VC1D_E_ALIAS;
     }
     if (a->dinitial != nullptr) {

@@ -53,8 +53,6 @@ def _check_decay(log_decay: torch.Tensor, heads: int, device) -> torch.Tensor:
         raise ValueError(f"log_decay shape {tuple(log_decay.shape)} does not match the {heads} heads")
     if log_decay.dtype != torch.float32:
         raise ValueError(f"log_decay must be float32, got {log_decay.dtype}")
-    if log_decay.requires_grad and torch.is_grad_enabled():
-        raise ValueError("log_decay is fixed: it has no gradient (pass log_decay.detach())")
     _require_cuda(log_decay, "log_decay")
     _same_device(log_decay, device, "log_decay")
     return log_decay.contiguous()
@@ -158,7 +156,7 @@ def _forward(q, k, v, log_decay, seq_idx, initial_states, return_final_states, f
              kernel, segments):
     want_state = bool(return_final_states) or final_states_out is not None
     plain = out is None and final_states_out is None and q.is_cuda and (seq_idx is None or seq_idx.dtype == torch.int32) \
-        and log_decay.is_contiguous() and not (log_decay.requires_grad and torch.is_grad_enabled())
+        and log_decay.is_contiguous()
     key = None
     if plain:
         key = (_signature(q), _signature(k), _signature(v), _signature(log_decay), _signature(seq_idx),
@@ -262,6 +260,8 @@ def linear_attention_fn(
 
     Differentiable in q, k, v and initial_states, through o and the final state (``linear_attention_bwd``).
     """
+    if torch.is_grad_enabled() and log_decay.requires_grad:
+        raise ValueError("log_decay is fixed: it has no gradient (pass log_decay.detach())")
     if torch.compiler.is_compiling():
         if out is not None or final_states_out is not None:
             raise ValueError("out= / final_states_out= cannot be used under torch.compile")
@@ -398,10 +398,11 @@ def linear_attention_update(
 
 
 def _update(q, k, v, state, log_decay, attention_mask, scale, out):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
+                                    or log_decay.requires_grad):
         raise ValueError("linear_attention_update has no gradient: use linear_attention_fn with seqlen 1 and initial_states")
     key = None
-    if out is None and q.is_cuda and log_decay.is_contiguous() and not log_decay.requires_grad:
+    if out is None and q.is_cuda and log_decay.is_contiguous():
         key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype,
                v.get_device(), state.shape, state.stride(), state.dtype, state.get_device(), log_decay.shape, log_decay.dtype,
                log_decay.get_device(), _signature(attention_mask), scale)

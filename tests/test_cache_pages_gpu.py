@@ -168,3 +168,23 @@ def test_pages_far_apart():
     want = O.move_pages([t], [2, 0, 1])
     V.reorder_pages([t], torch.tensor([2, 0, 1], device=DEV))
     same([t], want)
+
+
+def test_large_tables_refuse_before_anything_moves():
+    """More tensors than one launch takes: what one launch refuses is refused across launches too, and nothing has moved."""
+    states = [torch.full((4, 8), float(n), device=DEV) + torch.arange(4, device=DEV)[:, None] for n in range(_cabi.PAGES_MAX_TENSORS + 3)]
+    idx = torch.tensor([1, 0, 3, 2], device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        V.reorder_pages(states + [states[0]], idx)
+    own = torch.tensor([1, 0, 3, 2], dtype=torch.int64, device=DEV)
+    table = V.PageTable(states + [own.view(4, 1)])
+    before = [t.clone() for t in states]
+    with pytest.raises(ValueError, match="among the pages"):
+        table.reorder(own)
+    with pytest.raises(ValueError, match="among the pages"):
+        table.copy(own[:2], own[2:])
+    torch.cuda.synchronize()
+    same(states, before)
+    want = O.move_pages(states + [own.view(4, 1)], idx.cpu())
+    table.reorder(idx)
+    same(states + [own.view(4, 1)], want)

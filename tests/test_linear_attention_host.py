@@ -52,6 +52,41 @@ def test_update_refusals():
         V.linear_attention_update(q[0], k, v, s, torch.zeros(2))
 
 
+def test_a_scale_held_on_the_device_is_refused():
+    """Its value could change between two calls of the same arguments, and it could want a gradient."""
+    q, k, v = qkv()
+    g, scale, state = torch.zeros(2), torch.tensor(0.5), torch.zeros(1, 2, 8, 8)
+    for call in (lambda: V.linear_attention_fn(q, k, v, g, scale=scale), lambda: V.linear_attention_bwd(q, k, v, g, v, scale=scale),
+                 lambda: V.linear_attention_update(q[:, 0], k[:, 0], v[:, 0], state, g, scale=scale)):
+        with pytest.raises(TypeError, match="scale must be a number"):
+            call()
+
+
+def test_overlapping_states_of_large_tables():
+    """Tables of more tensors than one launch takes are looked over as a whole, against all pairs byte by byte."""
+    from viby_model_b200.cache_pages import _check_apart
+
+    def shared(table, pages):
+        seen = set()
+        for base, size, stride in table:
+            mine = {base + i * stride + j for i in range(pages) for j in range(size)}
+            if seen & mine:
+                return True
+            seen |= mine
+        return False
+
+    # layers side by side in one pool, given twice, one byte too long at the front, in the middle, at the end, empty ones
+    pool = [(16 * n, 16, 160) for n in range(10)]
+    for table in (pool, pool[::-1], pool + [(160 * 4, 16, 16)], pool + [pool[3]], [(0, 17, 160)] + pool[1:], pool[:9] + [(144, 17, 160)],
+                  pool[:4] + [(64, 17, 160)] + pool[5:], pool + [(32, 0, 160)], [(0, 16, 16), (64, 16, 16), (128, 4, 4)],
+                  [(0, 16, 16), (63, 16, 16)], [(0, 400, 400), (100, 8, 8), (1600, 8, 8)]):
+        if shared(table, 4):
+            with pytest.raises(ValueError, match="overlap"):
+                _check_apart(table, 4)
+        else:
+            _check_apart(table, 4)
+
+
 def test_page_refusals():
     s = torch.zeros(4, 3)
     with pytest.raises(ValueError, match="CUDA device"):

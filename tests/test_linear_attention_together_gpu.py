@@ -265,3 +265,26 @@ def test_repeated_calls_with_other_data_alignment_and_devices_of_the_same_signat
         state = s0.to(DEV)
         V.linear_attention_update(args[0][:, 0], args[1][:, 0], args[2][:, 0], state, g)
     assert want[0].shape == o.shape
+
+
+def test_calls_without_tokens_are_remembered_too():
+    """Empty tensors have no address.  A thread of its own starts without prepared calls, whatever ran before."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def calls():
+        g = torch.full((2,), -0.1, device=DEV)
+        for dtype in (torch.float32, torch.bfloat16):
+            for shape in ((2, 0, 2, 16), (0, 5, 2, 16), (2, 3, 2, 16)):
+                x = torch.ones(shape, device=DEV, dtype=dtype)
+                for _ in range(3):
+                    o, s = V.linear_attention_fn(x, x, x, g, None, None, True)
+                    assert tuple(o.shape) == shape and bool(s.any()) == (x.numel() > 0)
+                    assert x.numel() == 0 or bool(o.any())
+                if shape[1] == 0 or shape[0] == 0:
+                    s = torch.ones(shape[0], 2, 16, 16, device=DEV)
+                    for _ in range(2):
+                        assert torch.equal(V.linear_attention_fn(x, x, x, g, None, s, True)[1], s)
+        return True
+
+    with ThreadPoolExecutor(1) as pool:
+        assert pool.submit(calls).result()

@@ -25,6 +25,19 @@ _nbytes, _requires_grad = attrgetter("nbytes"), attrgetter("requires_grad")
 _INDEX_DTYPES = {torch.int32: _cabi.VC1D_I32, torch.int64: _cabi.VC1D_I64}
 
 
+def _check_apart(table, pages: int) -> None:
+    """Refuses tensors ``(address, bytes of a page, bytes from page to page)`` that share a byte."""
+    ends = sorted((base, base + (pages - 1) * stride + size, size, stride) for base, size, stride in table if size > 0 and pages > 0)
+    open_ = []  # tensors that reach beyond the start of the next one: the layers of one pool
+    for a in ends:
+        open_ = [b for b in open_ if b[1] > a[0]]
+        for b in open_:
+            d = (a[0] - b[0]) % a[3]
+            if a[3] != b[3] or d < b[2] or d + a[2] > a[3]:  # equal strides: the pages interleave, or not
+                raise ValueError("states overlap: a tensor is given twice, or two share memory")
+        open_.append(a)
+
+
 class PageTable:
     """The pages of ``states``: tensors on one CUDA device with the same first dimension, each page contiguous (the
     distance between pages is free, so the layers of a pool ``[pages, layers, ...]`` may be given one by one), none
@@ -47,6 +60,8 @@ class PageTable:
             for n, t in enumerate(self.states):
                 table[3 * n: 3 * n + 3] = array("q", self._strided(t))
         self._table = table
+        if len(self.states) > _cabi.PAGES_MAX_TENSORS:  # a launch looks at its own tensors only
+            _check_apart(list(zip(table[0::3], table[1::3], table[2::3])), self.pages)
         if self.pages > _cabi.PAGES_MAX_PAGES:
             raise ValueError(f"at most {_cabi.PAGES_MAX_PAGES} pages, got {self.pages}")
 
@@ -78,6 +93,8 @@ class PageTable:
             if t is not None:
                 setattr(a, name, t.data_ptr())
         index = source if source is not None else dst
+        if len(self.states) > _cabi.PAGES_MAX_TENSORS:  # refused before the first launch, not between two
+            self._check_arrays([t for t in (source, dst, live) if t is not None])
         if index is not None:
             a.index_dtype = _INDEX_DTYPES[index.dtype]
         stream = _stream_handle(self.device)
@@ -97,6 +114,14 @@ class PageTable:
             if other:
                 torch.cuda.set_device(prev)
         torch.autograd.graph.increment_version(self.states)  # a graph that saved one of them refuses to run
+
+    def _check_arrays(self, arrays) -> None:
+        table = self._table
+        for t in arrays:
+            lo, hi = t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+            for base, size, stride in zip(table[0::3], table[1::3], table[2::3]):
+                if size > 0 and lo < base + (self.pages - 1) * stride + size and base < hi:
+                    raise ValueError("an index tensor lies among the pages that are moved")
 
     def _index(self, t: torch.Tensor, what: str) -> torch.Tensor:
         if not isinstance(t, torch.Tensor) or t.dim() != 1:

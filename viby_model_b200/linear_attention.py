@@ -58,6 +58,12 @@ def _check_decay(log_decay: torch.Tensor, heads: int, device) -> torch.Tensor:
     return log_decay.contiguous()
 
 
+def _check_scale(scale) -> None:
+    """A tensor's value is on the device, may change between two calls, and would want a gradient."""
+    if isinstance(scale, torch.Tensor):
+        raise TypeError("scale must be a number, got a tensor")
+
+
 def _changed(*tensors) -> None:
     """Tells autograd that the tensors were written in place: a graph that saved one of them then refuses to run."""
     torch.autograd.graph.increment_version([t for t in tensors if t is not None])
@@ -65,6 +71,10 @@ def _changed(*tensors) -> None:
 
 def _signature(t: Optional[torch.Tensor]):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _aligned(q, k, v) -> bool:
+    return not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15
 
 
 # Prepared argument structs by call signature (shapes, strides, dtypes, devices, options), per host thread: a repeated call
@@ -190,7 +200,7 @@ def _forward(q, k, v, log_decay, seq_idx, initial_states, return_final_states, f
     _cabi.check(st, "linear_attention_fn")
     _changed(out, state)
     # workspace sizes and kernels depend on the alignment of the data too: only aligned calls are remembered, for aligned calls
-    if key is not None and len(_prepared("linear_args")) < 256 and not (a.q | a.k | a.v) & 15:
+    if key is not None and len(_prepared("linear_args")) < 256 and _aligned(q, k, v):
         _prepared("linear_args")[key] = (a, 0 if ws is None else ws.numel())
     del keep, ws
     return out, state
@@ -212,7 +222,7 @@ def _run_prepared(a, ws_bytes, q, k, v, log_decay, seq_idx, initial_states, atte
     if want_state:
         state = torch.empty((a.batch, a.heads, a.dim_k, a.dim_v), dtype=torch.float32, device=device)
         a.final_state = state.data_ptr()
-    if (a.q | a.k | a.v) & 15:  # another kernel, maybe with a workspace of its own size
+    if not _aligned(q, k, v):  # another kernel, maybe with a workspace of its own size
         ws = _workspace(a, _cabi.lib.vc1d_linear_workspace, device)
     else:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
@@ -255,11 +265,12 @@ def linear_attention_fn(
         overlap ``initial_states``).
       attention_mask ``[batch, seqlen]`` (bool / int / float; nonzero = valid): a masked token is not read, leaves the state
         as it is (no decay either) and its output is 0.
-      scale: ``dim_k ** -0.5`` by default.
-      kernel: None, "simt" or "mma"; segments: parts of the time axis (0 = automatic), for benches and tests.
+      scale: a number, ``dim_k ** -0.5`` by default.
+      kernel: None, "simt", "mma" or "tc"; segments: parts of the time axis (0 = automatic), for benches and tests.
 
     Differentiable in q, k, v and initial_states, through o and the final state (``linear_attention_bwd``).
     """
+    _check_scale(scale)
     if torch.is_grad_enabled() and log_decay.requires_grad:
         raise ValueError("log_decay is fixed: it has no gradient (pass log_decay.detach())")
     if torch.compiler.is_compiling():
@@ -304,6 +315,7 @@ def linear_attention_bwd(
     """Gradients of ``linear_attention_fn``: ``(dq, dk, dv, dinitial)`` for the gradient ``dout`` of its output and,
     where the final state was used, ``dfinal_states`` of that.  ``dinitial`` (fp32) is None unless ``need_dinitial``
     (default: when ``initial_states`` is given).  Gradients of shared key / value heads are summed over their heads."""
+    _check_scale(scale)
     if need_dinitial is None:
         need_dinitial = initial_states is not None
     if seq_idx is not None and (attention_mask is not None or initial_states is not None or dfinal_states is not None or need_dinitial):
@@ -389,6 +401,7 @@ def linear_attention_update(
     ``[batch, heads, dim_k, dim_v]`` as ``linear_attention_fn`` returns it (a slice ``pool[:n]`` of a larger pool too).
     ``attention_mask[batch]``: rows whose value is 0 (idle slots of a captured decode step) keep their state untouched
     and get zeros.  No gradient: for one differentiable token call ``linear_attention_fn`` with ``seqlen`` 1."""
+    _check_scale(scale)
     if torch.compiler.is_compiling():
         if out is not None:
             raise ValueError("out= cannot be used under torch.compile")

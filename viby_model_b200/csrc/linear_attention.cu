@@ -1,5 +1,6 @@
 // Linear attention: checks of arguments, how the time axis is split, and the runs that make up a forward or backward
-// pass (linear_attention.cuh).  The products live in linear_attention_simt.cu and linear_attention_mma.cu.
+// pass (linear_attention.cuh).  The products live in linear_attention_simt.cu, linear_attention_mma.cuh and
+// linear_attention_tc.cuh.
 #include <algorithm>
 
 #include "linear_attention.cuh"

@@ -4,6 +4,10 @@
 // One CTA of 256 threads owns one (row, head, slab of 64 state columns, part of the time axis) and walks its chunks of
 // 64 tokens.  q, k, v (converted to fp32), the state slab and the 64 x 64 products sit in shared memory; every product
 // is a register tile of 4 x 4 outputs per thread, fed by 128-bit shared loads (8 of them per 64 multiply-adds).
+//
+// Bound by those shared loads and by latency: a forward and backward pass over 3 x 777 tokens of 6 heads of 72 and 88 takes
+// 430 us in fp32, where memory would allow 2.5: 18 (row, head) pairs and two slabs for 148 SMs, so that the time axis is split
+// and every part computed twice over, once for its state.
 #include "linear_attention.cuh"
 
 namespace vc1d {

@@ -12,15 +12,24 @@
 // Six groups of four warps, each with its own part, chunk after chunk, linked by mbarriers only:
 //     warps 0-3    decays of P and its operand for the keys 0-63, then the columns 0-31 of the output
 //     warps 4-7    the state: X = a^n X + KV, and its bf16 copy in shared memory   (rows 128-159: warp 22)
-//     warps 8-15   the weighted values, split into three parts
-//     warps 16-19  the same for the keys 64-127 and the columns 32-63
-//     warp 20      issues the products
-//     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
-//     warp 23      says which tokens of a chunk count; where there is a mask, clears the rows of masked ones, whatever they
-//                  hold, and hands the chunk over
+//     warps 8-15   the weighted values, split into three parts; in two halves of 64 tokens, so that the products with one
+//                  and the weighing of the other overlap
+//     warps 16-19  the same as 0-3 for the keys 64-127 and the columns 32-63
+//     warp 20      issues the products for the outputs
+//     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's) and says
+//                  which of them count; where there is a mask, clears the rows of masked ones, whatever they hold, and
+//                  hands the chunk over
+//     warp 23      issues the products for the state
 // The parts are short programs of a few hundred instructions at five or so cycles each, so it is the longest part that
-// sets the pace: that is why there are so many, and twice the warps for the weighted values.
+// sets the pace: that is why there are so many, and twice the warps for the weighted values.  Two warps issue products
+// because a wait costs some 300 cycles while the tensor cores load shared memory, and one warp's waits then leave them idle
+// (one issuing warp for all: 65536 tokens of 16 heads of 128 took 680 us, now 605).
 // While one chunk's P is being decayed, the next chunk's tokens arrive and the state runs ahead.
+//
+// What bounds it: shared memory.  A chunk of 128 state rows moves some 440 KB through it (KV reads k^T three times, once
+// for each part), 3400 cycles of the 5000 that a chunk takes; with 160 rows it is 620 KB, 4900 of 9000.  The fp32 state,
+// its three-part products and the split in slabs of 64 columns (q and k are read once for each slab) cost more than the
+// products themselves: the tensor cores work for less than a third of the time, HBM for a sixth.
 //
 // Shared memory holds every operand as panels of 64 channels: rows of 128 bytes with the 16-byte units XORed by the row
 // modulo 8 (the 128-byte swizzle of the matrix descriptors).  A panel serves as K-major (channels summed: q, k) and as
@@ -593,32 +602,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             // in two halves, so that the products with one and the weighing of the other overlap
 #pragma unroll 1
             for (int half = 0; half < 2; ++half) {
-            if (half && ch >= kBack) ok = ok && wait(kKvDone, ch - kBack);
+                if (half && ch >= kBack) ok = ok && wait(kKvDone, ch - kBack);
 #pragma unroll
-            for (int i = 2 * half; i < 2 * half + 2; ++i) {
-                const int tok = (me >> 3) + kWeighers / 8 * i;
-                const uint4 in = *reinterpret_cast<const uint4*>(v + tok * 128 + at);
-                const float2 wt = make_float2(add[tok], add[tok]);
-                const uint32_t e[4] = {in.x, in.y, in.z, in.w};
-                uint32_t part[3][4];
+                for (int i = 2 * half; i < 2 * half + 2; ++i) {
+                    const int tok = (me >> 3) + kWeighers / 8 * i;
+                    const uint4 in = *reinterpret_cast<const uint4*>(v + tok * 128 + at);
+                    const float2 wt = make_float2(add[tok], add[tok]);
+                    const uint32_t e[4] = {in.x, in.y, in.z, in.w};
+                    uint32_t part[3][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float2 x = mul2(make_float2(__uint_as_float(e[j] << 16), __uint_as_float(e[j] & 0xffff0000u)), wt);
-                    // three parts cut off the top, eight bits each: nothing of the 24 is lost
+                    for (int j = 0; j < 4; ++j) {
+                        float2 x = mul2(make_float2(__uint_as_float(e[j] << 16), __uint_as_float(e[j] & 0xffff0000u)), wt);
+                        // three parts cut off the top, eight bits each: nothing of the 24 is lost
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        part[p][j] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
-                        if (p < 2)
-                            x = fma2(make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u)),
-                                     make_float2(-1.f, -1.f), x);
+                        for (int p = 0; p < 3; ++p) {
+                            part[p][j] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+                            if (p < 2)
+                                x = fma2(make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u)),
+                                         make_float2(-1.f, -1.f), x);
+                        }
                     }
-                }
 #pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    *reinterpret_cast<uint4*>(w + p * kPanel + tok * 128 + at) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
-            }
-            fence_async_smem();
-            mbar_arrive(bar(kVwRdy + half, ch));
+                    for (int p = 0; p < 3; ++p)
+                        *reinterpret_cast<uint4*>(w + p * kPanel + tok * 128 + at) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+                }
+                fence_async_smem();
+                mbar_arrive(bar(kVwRdy + half, ch));
             }
         }
     } else {
@@ -773,6 +782,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 if (!ok) break;
             }
             if (more) {
+                // nobody looks at the chunk before the last but one any more
+                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) break;
+                ask(&m.v, nullptr, 2, 1, c0, head_v, base + L::kV + (ch & 1) * kPanel);
+                if (!STATES && NQ == 1 && ch == 0 && !ask_queries()) break;
                 // the tokens of the chunk that count, and the sequence starts in the run's order
                 unsigned vb[4], sb[4];
 #pragma unroll
@@ -787,9 +800,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                     vb[w] = __ballot_sync(0xffffffffu, v);
                     sb[w] = __ballot_sync(0xffffffffu, s);
                 }
-                // nobody looks at the chunk before the last but one any more
-                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) break;
-                ask(&m.v, nullptr, 2, 1, c0, head_v, base + L::kV + (ch & 1) * kPanel);
                 Info* f = infos + (ch & 3);
                 int n = 0, run = 0;
 #pragma unroll
@@ -814,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                     mbar_arrive(bar(kVFull, ch));
                 }
             }
-            if (more && !STATES && NQ == 1 && !ask_queries()) break;
+            if (more && !STATES && NQ == 1 && ch > 0 && !ask_queries()) break;
             __syncwarp();
         }
     }

@@ -12,24 +12,24 @@
 // Six groups of four warps, each with its own part, chunk after chunk, linked by mbarriers only:
 //     warps 0-3    decays of P and its operand for the keys 0-63, then the columns 0-31 of the output
 //     warps 4-7    the state: X = a^n X + KV, and its bf16 copy in shared memory   (rows 128-159: warp 22)
-//     warps 8-15   the weighted values, split into three parts; in two halves of 64 tokens, so that the products with one
-//                  and the weighing of the other overlap
-//     warps 16-19  the same as 0-3 for the keys 64-127 and the columns 32-63
-//     warp 20      issues the products for the outputs
-//     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's) and says
-//                  which of them count; where there is a mask, clears the rows of masked ones, whatever they hold, and
-//                  hands the chunk over
-//     warp 23      issues the products for the state
+//     warps 8-15   the weighted values, split into three parts
+//     warps 16-19  the same for the keys 64-127 and the columns 32-63
+//     warp 20      issues the products
+//     warp 21      brings tokens in by TMA (the 128-byte swizzle and the zeros past the last token are the copy's)
+//     warp 23      says which tokens of a chunk count; where there is a mask, clears the rows of masked ones, whatever they
+//                  hold, and hands the chunk over
 // The parts are short programs of a few hundred instructions at five or so cycles each, so it is the longest part that
-// sets the pace: that is why there are so many, and twice the warps for the weighted values.  Two warps issue products
-// because a wait costs some 300 cycles while the tensor cores load shared memory, and one warp's waits then leave them idle
-// (one issuing warp for all: 65536 tokens of 16 heads of 128 took 680 us, now 605).
+// sets the pace: that is why there are so many, and twice the warps for the weighted values.
 // While one chunk's P is being decayed, the next chunk's tokens arrive and the state runs ahead.
 //
-// What bounds it: shared memory.  A chunk of 128 state rows moves some 440 KB through it (KV reads k^T three times, once
-// for each part), 3400 cycles of the 5000 that a chunk takes; with 160 rows it is 620 KB, 4900 of 9000.  The fp32 state,
-// its three-part products and the split in slabs of 64 columns (q and k are read once for each slab) cost more than the
-// products themselves: the tensor cores work for less than a third of the time, HBM for a sixth.
+// What bounds it: shared memory and the chain of a chunk.  A chunk of 128 state rows moves some 440 KB through shared memory
+// (KV reads k^T three times, once for each part), 3400 cycles of the 5300 that a chunk takes; with 160 rows it is 620 KB,
+// 4900 of 7200 to 9000.  The tensor cores work for less than a third of the time, HBM for a sixth.  8 x 1024 tokens of 16
+// heads of 128: 79 us (the warp-level kernel: 134); 64 x 1024 of 4 heads of 128: 128 us, of 160: 247 us; 65536 tokens of
+// 16 heads of 128: 641 us, 0.25 of the rate that memory would allow.
+// Measured and not taken: a second warp that issues products, weighing in two halves, a second buffer of keys for 160
+// rows (their last 32 channels as half a panel).  Together they gave 608 us for the last of these, but a training step of
+// padded rows of 160 took 1060 us instead of 1005, because the warp that clears masked rows then also asks for tokens.
 //
 // Shared memory holds every operand as panels of 64 channels: rows of 128 bytes with the 16-byte units XORed by the row
 // modulo 8 (the 128-byte swizzle of the matrix descriptors).  A panel serves as K-major (channels summed: q, k) and as
@@ -70,7 +70,7 @@ constexpr unsigned kSpin = 1u << 22;  // polls of 64 ns and more
 constexpr uint32_t kTmP = 0, kTmOi = 256, kTmOa = 320, kTmKV = 384, kTmKV2 = 448, kTmCols = 512;
 __host__ __device__ constexpr uint32_t operand_column(int blk) { return (blk >> 1) * 64 + (blk & 1) * 16; }  // of 32 keys
 
-enum Bar { kTmaQ, kTmaK, kTmaV, kQFull, kKFull, kVFull, kPRaw, kPRdy, kVwRdy, kVwRdy2, kKvHalf, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
+enum Bar { kTmaQ, kTmaK, kTmaV, kQFull, kKFull, kVFull, kPRaw, kPRdy, kVwRdy, kKvDone, kKvFree, kXRdy, kQxDone, kPvDone, kOFree, kBars };
 
 struct Info {  // of a chunk's tokens, bit i of word i / 32 for token i; a ring of four
     unsigned valid[4], start[4];
@@ -78,26 +78,22 @@ struct Info {  // of a chunk's tokens, bit i of word i / 32 for token i; a ring 
     int n_before[4], run_before[4];  // in the words below
 };
 struct Maps {
-    CUtensorMap a, k, v, a_half, k_half;  // the last two: the half panel
+    CUtensorMap a, k, v;
 };
 struct AllMaps {
     Maps run[kMaxRuns];
 };
 
-// Of 160 channels the last 32 make a panel of half the width (rows of 64 bytes, the 64-byte swizzle): that is what makes
-// room for a second buffer of keys.
-template <int ROWS, bool STATES>
+template <int ROWS>
 struct Layout {
-    static constexpr bool kHalf = ROWS % 64 != 0;
-    static constexpr int kPanels = ROWS / 64 + kHalf;
-    static constexpr int kStage = ROWS * 2 * kC;        // bytes of a chunk's queries or keys
-    static constexpr int kQStages = kHalf ? 1 : 2;      // keys and values have two
+    static constexpr int kPanels = ROWS / 64 + (ROWS % 64 != 0);
+    static constexpr int kStages = ROWS <= 128 ? 2 : 1;  // of q and k; v has two
     static constexpr int kQ = 0;
-    static constexpr int kK = kQ + (STATES ? 3 * kPanel : kQStages * kStage);
-    static constexpr int kV = kK + 2 * kStage;
+    static constexpr int kK = kQ + kStages * kPanels * kPanel;
+    static constexpr int kV = kK + kStages * kPanels * kPanel;
     static constexpr int kW = kV + 2 * kPanel;
     static constexpr int kX = kW + 3 * kPanel;
-    static constexpr int kBlock = kX + (STATES ? 0 : ROWS * 128);
+    static constexpr int kBlock = kX + ROWS * 128;
     static constexpr int kPowers = kBlock + 256;  // 32 zeros before them
     static constexpr int kAdd = kPowers + 8 * kPow;
     static constexpr int kWhole = kAdd + 4 * kC;  // bit per chunk: no token is masked
@@ -110,9 +106,6 @@ struct Layout {
 // ---- tcgen05 ----
 __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
     return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
-__device__ __forceinline__ uint64_t desc_half(uint32_t addr, uint32_t lbo) {  // the 64-byte swizzle: 8 rows are 512 bytes
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(512 >> 4) << 32 | 1ull << 46 | 4ull << 61;
 }
 // the same matrix `bytes` further
 __device__ __forceinline__ uint64_t at(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
@@ -215,10 +208,10 @@ __device__ __forceinline__ bool poll(uint32_t addr, uint32_t parity, volatile ui
 // the hot code of all parts together has to stay in the SM's instruction cache.
 template <int ROWS, bool STATES, bool REV>
 __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant__ Launch l, const __grid_constant__ AllMaps maps, unsigned int* timeouts) {
-    using L = Layout<ROWS, STATES>;
+    using L = Layout<ROWS>;
     using T = __nv_bfloat16;
-    constexpr int NQ = L::kQStages;
-    constexpr bool kSecond = L::kHalf;  // warp 22 holds rows 128 and up
+    constexpr int NS = L::kStages;
+    constexpr bool kSecond = ROWS > 128;  // warp 22 holds rows 128 and up
     extern __shared__ __align__(1024) unsigned char sm[];  // the swizzle goes by address: panels start at multiples of 1024
     const uint32_t base = smem_u32(sm);
     float* block = reinterpret_cast<float*>(sm + L::kBlock);  // a^31 .. a^0; a^0 .. a^31 in a reversed run
@@ -271,11 +264,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         if (n < 32) block[rev ? n : 31 - n] = hi, pw_hi[n - 32] = 0.f;
     }
     // panels of k that the head does not reach are read as rows of the state all the same; every other byte is written first
-    for (int i = (r.da + 63) / 64 * kPanel + tid * 16; i < L::kStage; i += kThreads * 16)
-        for (int n = 0; n < 2; ++n) *reinterpret_cast<uint4*>(sm + L::kK + n * L::kStage + i) = make_uint4(0, 0, 0, 0);
-    const uint32_t last = base + L::kMisc + 8;  // see the end
+    for (int p = (r.da + 63) / 64; p < L::kPanels; ++p)
+        for (int i = tid; i < NS * kPanel / 16; i += kThreads)
+            *reinterpret_cast<uint4*>(sm + L::kK + (i / (kPanel / 16) * L::kPanels + p) * kPanel + i % (kPanel / 16) * 16) = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
-        mbar_init(last, 2);
         misc[1] = misc[4] = misc[5] = misc[6] = 0;
         for (int i = 0; i < 2; ++i) {
             for (int x = 0; x < 3; ++x) {
@@ -285,8 +277,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             mbar_init(bar(kPRaw, i), 2);   // the products, and the chunk's info
             mbar_init(bar(kPRdy, i), 256);
             mbar_init(bar(kVwRdy, i), kWeighers);
-            mbar_init(bar(kVwRdy2, i), kWeighers);
-            mbar_init(bar(kKvHalf, i), 1);
             mbar_init(bar(kKvDone, i), 2);
             mbar_init(bar(kKvFree, i), kSecond ? 160 : 128);
             mbar_init(bar(kXRdy, i), kSecond ? 160 : 128);
@@ -583,11 +573,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         // ------------------------------------------------------------------------------ weighted values
         few_registers();
         const int me = tid - 256;
-        bool ok = true;
 #pragma unroll 1
         for (int ch = 0; ch < chunks; ++ch) {
             constexpr int kBack = STATES ? 2 : 1;  // buffers
-            ok = ok && wait(kVFull, ch) && (ch < kBack || wait(kKvHalf, ch - kBack));
+            const bool ok = wait(kVFull, ch) && (ch < kBack || wait(kKvDone, ch - kBack));
             if (!all_of(1, kWeighers, ok)) break;  // the weights of the chunk before are no longer read
             const Info& f = infos[ch & 3];
             if (me < kC) {
@@ -599,244 +588,211 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
             const unsigned char* v = sm + L::kV + (ch & 1) * kPanel;
             unsigned char* w = sm + weighted(ch);
             const int at = ((me & 7) ^ (me >> 3 & 7)) << 4;  // rows 32 apart have the same swizzle
-            // in two halves, so that the products with one and the weighing of the other overlap
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                if (half && ch >= kBack) ok = ok && wait(kKvDone, ch - kBack);
+#pragma unroll 2
+            for (int i = 0; i < kC * 8 / kWeighers; ++i) {
+                const int tok = (me >> 3) + kWeighers / 8 * i;
+                const uint4 in = *reinterpret_cast<const uint4*>(v + tok * 128 + at);
+                const float2 wt = make_float2(add[tok], add[tok]);
+                const uint32_t e[4] = {in.x, in.y, in.z, in.w};
+                uint32_t part[3][4];
 #pragma unroll
-                for (int i = 2 * half; i < 2 * half + 2; ++i) {
-                    const int tok = (me >> 3) + kWeighers / 8 * i;
-                    const uint4 in = *reinterpret_cast<const uint4*>(v + tok * 128 + at);
-                    const float2 wt = make_float2(add[tok], add[tok]);
-                    const uint32_t e[4] = {in.x, in.y, in.z, in.w};
-                    uint32_t part[3][4];
+                for (int j = 0; j < 4; ++j) {
+                    float2 x = mul2(make_float2(__uint_as_float(e[j] << 16), __uint_as_float(e[j] & 0xffff0000u)), wt);
+                    // three parts cut off the top, eight bits each: nothing of the 24 is lost
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float2 x = mul2(make_float2(__uint_as_float(e[j] << 16), __uint_as_float(e[j] & 0xffff0000u)), wt);
-                        // three parts cut off the top, eight bits each: nothing of the 24 is lost
-#pragma unroll
-                        for (int p = 0; p < 3; ++p) {
-                            part[p][j] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
-                            if (p < 2)
-                                x = fma2(make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u)),
-                                         make_float2(-1.f, -1.f), x);
-                        }
+                    for (int p = 0; p < 3; ++p) {
+                        part[p][j] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+                        if (p < 2)
+                            x = fma2(make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u)),
+                                     make_float2(-1.f, -1.f), x);
                     }
-#pragma unroll
-                    for (int p = 0; p < 3; ++p)
-                        *reinterpret_cast<uint4*>(w + p * kPanel + tok * 128 + at) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
                 }
-                fence_async_smem();
-                mbar_arrive(bar(kVwRdy + half, ch));
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<uint4*>(w + p * kPanel + tok * 128 + at) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
             }
+            fence_async_smem();
+            mbar_arrive(bar(kVwRdy, ch));
         }
     } else {
         many_registers();  // the same instruction for the four warps of the group
-        const bool leader = elect_lane();
-        // ------------------------------------------------------------------------------ products for the outputs
+        // ------------------------------------------------------------------------------ products
         if (warp == 20) {
+            const bool leader = elect_lane();
             const int steps = (r.da + 15) / 16;
             const uint32_t q0 = base + L::kQ, k0 = base + L::kK, v0 = base + L::kV, x0 = base + L::kX;
-            // step s of a product over channels
-            auto channels = [&](uint32_t addr, uint64_t d, int s) {
-                return s < 8 ? at(d, (s >> 2) * kPanel + (s & 3) * 32) : at(desc_half(addr + 2 * kPanel, 16), (s & 1) * 32);
-            };
             auto products_of_keys = [&](int ch) {  // P of a chunk
                 if (!wait_warp(kKFull, ch) || !wait_warp(kQFull, ch)) return false;
                 fence_after();
-                const uint32_t q = q0 + (ch % NQ) * L::kStage, k = k0 + (ch & 1) * L::kStage;
-                const uint64_t dq = desc_k(q), dk = desc_k(k);
+                const uint64_t dq = desc_k(q0 + (ch % NS) * L::kPanels * kPanel), dk = desc_k(k0 + (ch % NS) * L::kPanels * kPanel);
                 const uint32_t d = tm + kTmP + (ch & 1) * 128;
 #pragma unroll
                 for (int s = 0; s < ROWS / 16; ++s)
-                    if (s < steps) mma_ss(leader, d, channels(q, dq, s), channels(k, dk, s), idesc(128, false, false), s > 0);
+                    if (s < steps) mma_ss(leader, d, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dk, (s >> 2) * kPanel + (s & 3) * 32), idesc(128, false, false), s > 0);
                 commit(leader, bar(kPRaw, ch));
                 return true;
             };
-            auto inside_chunk = [&](int ch) {
-                if (!wait_warp(kPRdy, ch)) return false;
-                fence_after();
-                const uint64_t dv = desc_mn(v0 + (ch & 1) * kPanel);
-#pragma unroll
-                for (int s = 0; s < kC / 16; ++s)
-                    mma_ts(leader, tm + kTmOa, tm + kTmP + (ch & 1) * 128 + operand_column(s >> 1) + 8 * (s & 1), at(dv, s * 2048), idesc(kCols, false, true), s > 0);
-                commit(leader, bar(kPvDone, ch));
-                return true;
-            };
-            bool going = STATES || NQ == 1 || chunks == 0 || products_of_keys(0);
+            bool going = STATES || NS == 1 || chunks == 0 || products_of_keys(0);
 #pragma unroll 1
-            for (int ch = 0; !STATES && going && ch < chunks; ++ch) {
-                if (NQ == 1 && !products_of_keys(ch)) break;
-                if (!wait_warp(kXRdy, ch) || (ch > 0 && !wait_warp(kOFree, ch - 1))) break;
-                fence_after();
-                const uint32_t q = q0 + (ch % NQ) * L::kStage;
-                const uint64_t dq = desc_k(q), dx = desc_mn(x0);
-#pragma unroll
-                for (int s = 0; s < ROWS / 16; ++s)
-                    if (s < steps) mma_ss(leader, tm + kTmOi, channels(q, dq, s), at(dx, s * 2048), idesc(kCols, false, true), s > 0);
-                commit(leader, bar(kQxDone, ch));
-                // with two buffers of queries, the next chunk's products fill the time that this one's decays take
-                if (NQ == 2 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
-                if (!inside_chunk(ch)) break;
-            }
-        }
-        // ------------------------------------------------------------------------------ products for the state
-#pragma unroll 1
-        for (int ch = 0; warp == 23 && ch < chunks; ++ch) {
-            const uint32_t k = base + L::kK + (ch & 1) * L::kStage;
-            if (!wait_warp(kKFull, ch) || (ch > 0 && !wait_warp(kKvFree, ch - 1))) break;
-            bool ok = true;
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {  // tokens 0-63, then 64-127
-                ok = wait_warp(kVwRdy + half, ch);
-                if (!ok) break;
+            for (int ch = 0; going && ch < chunks; ++ch) {
+                const uint32_t q = q0 + (ch % NS) * L::kPanels * kPanel, k = k0 + (ch % NS) * L::kPanels * kPanel, v = v0 + (ch & 1) * kPanel;
+                if (!wait_warp(kKFull, ch) || !wait_warp(kVwRdy, ch) || (ch > 0 && !wait_warp(kKvFree, ch - 1))) break;
                 fence_after();
 #pragma unroll 1
-                for (int tile = 0; tile < (kSecond ? 2 : 1); ++tile) {
-                    // rows 0-127; then the half panel as the third group of 32 rows, where warp 22 can read them (what is
-                    // beside it gives rows that nobody reads)
-                    const int step = tile ? 1024 : 2048;
-                    const uint64_t dk = at(tile ? desc_half(k + kPanel, kPanel / 2) : desc_mn(k), half * 4 * step);
-                    uint64_t dw = desc_mn(base + weighted(ch) + 2 * kPanel + half * (kPanel / 2));
+                for (int tile = 0; tile < (kSecond ? 2 : 1); ++tile) {  // rows 0-127; 64-191, of which 128-159 are used
+                    const uint64_t dk = desc_mn(k + tile * kPanel);
+                    uint64_t dw = desc_mn(base + weighted(ch) + 2 * kPanel);
 #pragma unroll 1
                     for (int p = 2; p >= 0; --p) {
 #pragma unroll
-                        for (int s = 0; s < kC / 32; ++s)
-                            mma_ss(leader, tm + (tile ? kTmKV2 : kTmKV), at(dk, s * step), at(dw, s * 2048), idesc(kCols, true, true), half || p < 2 || s > 0);
+                        for (int s = 0; s < kC / 16; ++s) mma_ss(leader, tm + (tile ? kTmKV2 : kTmKV), at(dk, s * 2048), at(dw, s * 2048), idesc(kCols, true, true), p < 2 || s > 0);
                         dw -= kPanel >> 4;
                     }
                 }
-                commit(leader, bar(half ? kKvDone : kKvHalf, ch));
+                commit(leader, bar(kKvDone, ch));
+                if (!STATES) {
+                    // with one buffer of keys the state's products go first: theirs is the longer way to the next chunk
+                    if (NS == 1 && !products_of_keys(ch)) break;
+                    if (!wait_warp(kXRdy, ch) || (ch > 0 && !wait_warp(kOFree, ch - 1))) break;
+                    fence_after();
+                    const uint64_t dq = desc_k(q), dx = desc_mn(x0), dv = desc_mn(v);
+#pragma unroll
+                    for (int s = 0; s < ROWS / 16; ++s)
+                        if (s < steps) mma_ss(leader, tm + kTmOi, at(dq, (s >> 2) * kPanel + (s & 3) * 32), at(dx, s * 2048), idesc(kCols, false, true), s > 0);
+                    commit(leader, bar(kQxDone, ch));
+                    // the next chunk's products fill the time that this one's decays take
+                    if (NS == 2 && ch + 1 < chunks && !products_of_keys(ch + 1)) break;
+                    if (!wait_warp(kPRdy, ch)) break;
+                    fence_after();
+#pragma unroll
+                    for (int s = 0; s < kC / 16; ++s)
+                        mma_ts(leader, tm + kTmOa, tm + kTmP + (ch & 1) * 128 + operand_column(s >> 1) + 8 * (s & 1), at(dv, s * 2048), idesc(kCols, false, true), s > 0);
+                    commit(leader, bar(kPvDone, ch));
+                }
             }
-            if (!ok) break;
         }
         if (kSecond && warp == 22) state(128 + lane, kTmKV2);
         // ------------------------------------------------------------------------------ tokens
         const Maps& m = maps.run[blockIdx.z];
         const int panels = (r.da + 63) / 64;
+        const bool leader = elect_lane();
         if (warp == 21 && leader) {
             tma::prefetch_tensormap(&m.k);
             tma::prefetch_tensormap(&m.v);
             if (!STATES) tma::prefetch_tensormap(&m.a);
-            if (L::kHalf) {
-                tma::prefetch_tensormap(&m.k_half);
-                if (!STATES) tma::prefetch_tensormap(&m.a_half);
-            }
         }
         const int head_a = h / r.a.group, head_k = h / r.k.group, head_v = h / r.v.group;
-        auto all = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
 #pragma unroll 1
-        for (int ch = 0; warp == 21 && ch <= chunks; ++ch) {
-            const bool more = ch < chunks;
+        for (int ch = 0; warp == 21 && ch < chunks; ++ch) {
             const int t0 = first_token(ch);
-            const int hand_over = more && to_clear(ch) ? kTmaQ : kQFull;
-            auto ask = [&](const CUtensorMap* map, const CUtensorMap* half, int what, int n_panels, int c_first, int head, uint32_t to) {
+            const int hand_over = to_clear(ch) ? kTmaQ : kQFull;
+            auto ask = [&](const CUtensorMap* map, int what, int n_panels, int c_first, int head, uint32_t to) {
                 const uint32_t done = bar(hand_over + what, ch);
                 if (leader) {
-                    tma::mbar_arrive_expect_tx(done, n_panels * kPanel - (L::kHalf && n_panels == L::kPanels ? kPanel / 2 : 0));
+                    tma::mbar_arrive_expect_tx(done, n_panels * kPanel);
                     tma_load_4d(to, map, c_first, t0, head, b, done);
                 }
 #pragma unroll
                 for (int p = 1; p < L::kPanels; ++p)
-                    if (leader && p < n_panels) tma_load_4d(to + p * kPanel, L::kHalf && p + 1 == L::kPanels ? half : map, c_first + p * 64, t0, head, b, done);
+                    if (leader && p < n_panels) tma_load_4d(to + p * kPanel, map, c_first + p * 64, t0, head, b, done);
                 if (leader) {
                     // the other barrier goes through its phase of this chunk too: phases are counted in chunks
                     if (hand_over == kQFull && c.mask != nullptr) mbar_arrive(bar(kTmaQ + what, ch));
                     misc[4 + what] = ch + 1;
                 }
             };
-            auto ask_queries = [&]() {
-                if (!all(ch < NQ || wait(kQxDone, ch - NQ))) return false;
-                ask(&m.a, &m.a_half, 0, panels, 0, head_a, base + L::kQ + (ch % NQ) * L::kStage);
+            auto all = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
+            auto ask_values = [&]() {
+                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) return false;
+                ask(&m.v, 2, 1, c0, head_v, base + L::kV + (ch & 1) * kPanel);
                 return true;
             };
-            if (more) {
-                // Each is asked for when its buffer is free.
-                if (!all(ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPRaw, ch - 2))))) break;
-                ask(&m.k, &m.k_half, 1, panels, 0, head_k, base + L::kK + (ch & 1) * L::kStage);
-                if (!STATES && NQ == 2 && !ask_queries()) break;
+            // Values have two buffers, keys and queries as many as fit.  Each is asked for when its own is free: with two of
+            // each, keys first; with one, values, because the next chunk's wait for nothing else.
+            if (!all(ch < 2 || (wait(kKvDone, ch - 2) && wait(kKvFree, ch - 2) && (STATES || wait(kPRaw, ch - 2))))) break;
+            if (NS == 1) {
+                if (!ask_values()) break;
+                if (!all(ch < 1 || (wait(kKvDone, ch - 1) && (STATES || wait(kPRaw, ch - 1))))) break;
             }
-            if (ch > 0 && to_clear(ch - 1)) {
-                // Rows of the chunk before, which is on its way or there.  Not later: the values of this chunk wait for outputs of
-                // the chunk before it, whose products are issued after the first ones of the chunk that is cleared here.
-                const Info* f = infos + (ch - 1 & 3);
-                bool ok = true;
+            ask(&m.k, 1, panels, 0, head_k, base + L::kK + (ch % NS) * L::kPanels * kPanel);
+            if (!STATES) {
+                if (!all(ch < NS || wait(kQxDone, ch - NS))) break;
+                ask(&m.a, 0, panels, 0, head_a, base + L::kQ + (ch % NS) * L::kPanels * kPanel);
+            }
+            if (NS == 2 && !ask_values()) break;
+            __syncwarp();
+        }
 #pragma unroll 1
-                for (int turn = 0; turn < (STATES ? 2 : 3); ++turn) {  // in the order they are needed
-                    const int what = (1 + turn) % 3;  // 2: values, 1: keys, 0: queries
-                    ok = wait_warp(kTmaQ + what, ch - 1);
-                    if (!ok) break;
-                    unsigned char* to = sm + (what == 2 ? L::kV + (ch - 1 & 1) * kPanel : what == 1 ? L::kK + (ch - 1 & 1) * L::kStage : L::kQ + ((ch - 1) % NQ) * L::kStage);
+        for (int ch = 0; warp == 23 && ch < chunks; ++ch) {
+            // nobody looks at the chunk before the last but one any more
+            if (ch >= 2 && !(wait_warp(kKvFree, ch - 2) && (STATES || wait_warp(kPvDone, ch - 2)))) break;
+            const int t0 = first_token(ch);
+            // the tokens of the chunk that count, and the sequence starts in the run's order
+            Info* f = infos + (ch & 3);
+            int n = 0, run = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int t = t0 + 32 * w + lane;
+                bool v = t >= 0 && t < c.seqlen, s = false;
+                if (v && c.seq_idx != nullptr && (rev ? t + 1 < c.seqlen : t > 0)) {
+                    const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + (long long)t * c.seq_st;
+                    s = p[0] != (rev ? p[c.seq_st] : p[-c.seq_st]);
+                }
+                if (v && c.mask != nullptr) v = mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + (long long)t * c.mask_st);
+                const unsigned vb = __ballot_sync(0xffffffffu, v), sb = __ballot_sync(0xffffffffu, s);
+                if (lane == 0) {
+                    f->valid[w] = vb;
+                    f->start[w] = sb;
+                    f->n_before[w] = n;
+                    f->run_before[w] = run;
+                }
+                n += __popc(vb);
+                run += __popc(sb);
+            }
+            if (lane == 0) {
+                f->n_all = n;
+                f->run_all = run;
+            }
+            __syncwarp();
+            if (leader) {  // for those who wait for the products or the values
+                if (!STATES) mbar_arrive(bar(kPRaw, ch));
+                mbar_arrive(bar(kKvDone, ch));
+                mbar_arrive(bar(kVFull, ch));
+            }
+            if (!to_clear(ch)) continue;
+            bool ok = true;
+#pragma unroll 1
+            for (int turn = 0; turn < (STATES ? 2 : 3); ++turn) {  // in the order they are asked for
+                const int what = NS == 1 ? 2 - turn : (STATES ? 1 + turn : (turn + 1) % 3);  // 2: values, 1: keys, 0: queries
+                ok = wait_warp(kTmaQ + what, ch);
+                if (!ok) break;
+                {
+                    unsigned char* to = sm + (what == 2 ? L::kV + (ch & 1) * kPanel : (what == 1 ? L::kK : L::kQ) + (ch % NS) * L::kPanels * kPanel);
                     for (int row = lane >> 3; row < kC; row += 4) {  // eight lanes to a row
                         if (f->valid[row >> 5] >> (row & 31) & 1u) continue;
-                        for (int p = 0; p < (what == 2 ? 1 : panels); ++p) {
-                            const bool half = L::kHalf && p + 1 == L::kPanels;
-                            if (half && (lane & 4)) continue;
-                            *reinterpret_cast<uint4*>(to + p * kPanel + row * (half ? 64 : 128) + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
+                        for (int p = 0; p < (what == 2 ? 1 : panels); ++p)
+                            *reinterpret_cast<uint4*>(to + p * kPanel + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_async_smem();
-                    __syncwarp();
-                    if (leader) mbar_arrive(bar(kQFull + what, ch - 1));
-                }
-                if (!ok) break;
-            }
-            if (more) {
-                // nobody looks at the chunk before the last but one any more
-                if (!all(ch < 2 || STATES || wait(kPvDone, ch - 2))) break;
-                ask(&m.v, nullptr, 2, 1, c0, head_v, base + L::kV + (ch & 1) * kPanel);
-                if (!STATES && NQ == 1 && ch == 0 && !ask_queries()) break;
-                // the tokens of the chunk that count, and the sequence starts in the run's order
-                unsigned vb[4], sb[4];
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int t = t0 + 32 * w + lane;
-                    bool v = t >= 0 && t < c.seqlen, s = false;
-                    if (v && c.seq_idx != nullptr && (rev ? t + 1 < c.seqlen : t > 0)) {
-                        const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + (long long)t * c.seq_st;
-                        s = p[0] != (rev ? p[c.seq_st] : p[-c.seq_st]);
-                    }
-                    if (v && c.mask != nullptr) v = mask_valid(c.mask, c.mask_dtype, (long long)b * c.mask_sb + (long long)t * c.mask_st);
-                    vb[w] = __ballot_sync(0xffffffffu, v);
-                    sb[w] = __ballot_sync(0xffffffffu, s);
-                }
-                Info* f = infos + (ch & 3);
-                int n = 0, run = 0;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if (lane == 0) {
-                        f->valid[w] = vb[w];
-                        f->start[w] = sb[w];
-                        f->n_before[w] = n;
-                        f->run_before[w] = run;
-                    }
-                    n += __popc(vb[w]);
-                    run += __popc(sb[w]);
-                }
-                if (lane == 0) {
-                    f->n_all = n;
-                    f->run_all = run;
                 }
                 __syncwarp();
-                if (leader) {  // for those who wait for the products or the values
-                    if (!STATES) mbar_arrive(bar(kPRaw, ch));
-                    mbar_arrive(bar(kKvDone, ch));
-                    mbar_arrive(bar(kVFull, ch));
-                }
+                if (leader) mbar_arrive(bar(kQFull + what, ch));
             }
-            if (more && !STATES && NQ == 1 && ch > 0 && !ask_queries()) break;
-            __syncwarp();
+            if (!ok) break;
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
-    // After an expired wait products and copies may still be under way: they end by themselves, and TMEM and shared memory
-    // have to outlive them.  A barrier of its own for the products of both warps; the copies' barriers for the copies.
-    if (*dead && (warp == 20 || warp == 23)) commit(elect_lane(), last);
     if (warp == 20) {
         fence_after();
         if (*dead && lane == 0) {
+            // products and copies may still be under way: they end by themselves, and TMEM and shared memory have to
+            // outlive them.  A barrier of its own for the products; the copies' barriers for the copies.
+            const uint32_t last = base + L::kMisc + 8;
+            mbar_init(last, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            commit(true, last);
             for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
             for (int what = 0; what < 3; ++what) {
                 const int asked = misc[4 + what];
@@ -849,17 +805,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     }
 }
 
-// The tensor map of rows as [batch, head, token, channel] with boxes of 64 (half a panel: 32) channels x 128 tokens.
-inline bool encode(CUtensorMap* map, const Rows& r, int batch, int heads, int seqlen, int dim, bool half = false) {
+// The tensor map of rows as [batch, head, token, channel] with boxes of 64 channels x 128 tokens.
+inline bool encode(CUtensorMap* map, const Rows& r, int batch, int heads, int seqlen, int dim) {
     tma::EncodeFn enc = tma::encode_fn();
     if (enc == nullptr) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)seqlen, (cuuint64_t)(heads / r.group), (cuuint64_t)batch};
     cuuint64_t st[3] = {2 * (cuuint64_t)r.st, 2 * (cuuint64_t)r.sh, 2 * (cuuint64_t)r.sb};
     for (int i = 0; i < 3; ++i)
         if (dims[i + 1] == 1) st[i] = 1024;  // an extent of 1 makes its stride irrelevant, but the encoder wants a legal one
-    const cuuint32_t box[4] = {half ? 32u : 64u, kC, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, kC, 1, 1}, step[4] = {1, 1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(r.p), dims, st, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // rows whose tokens run backwards, in natural order again
@@ -871,7 +827,7 @@ inline Rows natural(Rows r, int seqlen, int eb) {
 
 template <int ROWS, bool STATES, bool REV>
 cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) {
-    constexpr int smem = Layout<ROWS, STATES>::kBytes;
+    constexpr int smem = Layout<ROWS>::kBytes;
     static_assert(smem <= 232448, "shared memory of an SM");
     Launch l = given;
     AllMaps maps;
@@ -888,8 +844,6 @@ cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) 
         Maps& m = maps.run[i];
         if (l.c.seqlen > 0 && !(encode(&m.a, r.a, l.c.batch, l.c.heads, l.c.seqlen, r.da) && encode(&m.k, r.k, l.c.batch, l.c.heads, l.c.seqlen, r.da) &&
                                 encode(&m.v, r.v, l.c.batch, l.c.heads, l.c.seqlen, r.dv)))
-            return cudaErrorNotSupported;
-        if (Layout<ROWS, STATES>::kHalf && l.c.seqlen > 0 && !(encode(&m.a_half, r.a, l.c.batch, l.c.heads, l.c.seqlen, r.da, true) && encode(&m.k_half, r.k, l.c.batch, l.c.heads, l.c.seqlen, r.da, true)))
             return cudaErrorNotSupported;
     }
     auto kernel = k_linear_tc<ROWS, STATES, REV>;

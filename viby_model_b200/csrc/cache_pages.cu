@@ -24,6 +24,12 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTensors = VC1D_PAGES_MAX_TENSORS;
 constexpr int kMaxPages = VC1D_PAGES_MAX_PAGES;
 
+// Dynamic shared memory of a launch: the list of moves, and a staging area.  48 KB keep four CTAs on an SM; many pages take
+// more, so that a strip is at least a 16-byte column of all of them.
+constexpr int moves_bytes(int pages) { return (4 * pages + 15) & ~15; }
+constexpr int staging_bytes(int pages) { return std::max(48 << 10, 16 * pages); }
+constexpr int kMostShared = moves_bytes(kMaxPages) + staging_bytes(kMaxPages);
+
 struct PTensor {
     char* base;
     long long page_bytes, stride;
@@ -285,10 +291,11 @@ VC1D_API int vc1d_pages(const vc1d_pages_args* a, void* stream) {
     p.pages = a->pages;
     p.n = a->n;
     p.wide_index = a->index_dtype == VC1D_I64;
-    // 48 KB keep four CTAs on an SM; many pages take more, so that a strip is at least a 16-byte column of all of them
-    p.stage_bytes = std::max(48 << 10, 16 * a->pages);
-    const int smem = ((4 * a->pages + 15) & ~15) + p.stage_bytes;
-    cudaError_t e = cudaFuncSetAttribute(k_pages, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    p.stage_bytes = staging_bytes(a->pages);
+    const int smem = moves_bytes(a->pages) + p.stage_bytes;
+    // The limit belongs to the function, not to the host thread: always the largest, or a call with few pages would lower
+    // it between another thread's call with many and its launch.
+    cudaError_t e = cudaFuncSetAttribute(k_pages, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) return (int)e;
     const int per_sm = std::max(1, std::min(4, (220 << 10) / (smem + 2048)));
     const long long most = std::max<long long>(1, p.sum_page_bytes / 128 + p.n_tensors);

@@ -247,6 +247,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_simt(const __grid_consta
     }
 }
 
+// Dynamic shared memory of a CTA whose state has `da` rows (a multiple of four).
+constexpr int shared_bytes(int da) {
+    return 4 * (kChunk * ((da > kChunk ? da : kChunk) + 4) + kChunk * (da + 4) + kChunk * kSlab + da * kSlab);
+}
+static_assert(shared_bytes(kMaxDim) + 4096 <= 232448, "shared memory of a CTA");
+
 template <int DT, bool STATES>
 cudaError_t launch(const Launch& l, cudaStream_t s) {
     int da = 0, slabs = 0;
@@ -254,10 +260,12 @@ cudaError_t launch(const Launch& l, cudaStream_t s) {
         da = max(da, (l.run[i].da + 3) & ~3);
         slabs = max(slabs, (l.run[i].dv + kSlab - 1) / kSlab);
     }
-    const size_t smem = sizeof(float) * ((size_t)kChunk * (max(da, kChunk) + 4) + (size_t)kChunk * (da + 4) + (size_t)kChunk * kSlab + (size_t)da * kSlab);
+    const int smem = shared_bytes(da);
     const long long blocks = (long long)l.c.batch * l.c.heads * slabs;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(k_linear_simt<DT, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // The limit belongs to the function, not to the host thread: always that of the largest heads, or a call with small ones
+    // would lower it between another thread's call and its launch.
+    cudaError_t e = cudaFuncSetAttribute(k_linear_simt<DT, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes(kMaxDim));
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)blocks, STATES ? l.c.segments - 1 : l.c.segments, l.runs);
     note_launch(STATES ? "linear_simt_states" : "linear_simt");

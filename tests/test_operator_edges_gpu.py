@@ -1,0 +1,33 @@
+"""Calls at the edges of what linear attention and cache pages accept: lengths past 2^25, no tokens, remembered call forms,
+derivatives that there are none of, waits that run out.  Small tolerances only where sums are involved (tests/linear_cases.py)."""
+import pytest
+import torch
+
+import viby_model_b200 as V
+from linear_cases import check, decays, magnitudes, make, tolerance
+from oracle import linear_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("side", ["left", "right"])
+def test_padding_of_more_than_2_to_the_25_tokens(side):
+    """One part of the time axis whose padding, times the 64 columns of a slab, does not fit 31 bits."""
+    T, D, n = (1 << 25) + 389, 8, 5
+    q, k, v = (torch.full((1, T, 1, D), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(3))
+    small = make(1, n, 1, 1, 1, D, D, torch.bfloat16)[:3]
+    at = slice(T - n, T) if side == "left" else slice(0, n)
+    for x, y in zip((q, k, v), small):
+        x[:, at] = y.to(DEV)
+    mask = torch.zeros(1, T, dtype=torch.bool, device=DEV)
+    mask[:, at] = True
+    out = torch.ones(1, T, 1, D, dtype=torch.bfloat16, device=DEV)
+    g = decays(1)
+    _, state = V.linear_attention_fn(q, k, v, g.to(DEV), return_final_states=True, attention_mask=mask, out=out, kernel="tc", segments=1)
+    ref, ref_s = O.linear_attention(*small, g)
+    M, M_s = magnitudes(*small, g)
+    check(out[:, at], ref, tolerance(ref, M, torch.bfloat16, D, n, True), "out")
+    check(state, ref_s, tolerance(ref_s, M_s, torch.bfloat16, D, n, True, torch.float32), "state")
+    out[:, at] = 0
+    assert not bool(out.view(torch.int32).any())  # +0, every one of them

@@ -321,8 +321,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         if (!STATES) {
             const int eb = r.out_f32 ? 4 : 2, before = max(0, min(t_end, t_begin + lo * kC) - t_begin), after = hi < 0 ? t_end : min(t_end, t_begin + (hi + 1) * kC);
             char* o = const_cast<char*>(static_cast<const char*>(r.o.p)) + ((long long)b * r.o.sb + (long long)h * r.o.sh + (long long)c0 * r.o.sd) * eb;
-            for (int i = tid; i < (before + t_end - after) * kCols; i += kThreads) {
-                const int row = i / kCols, col = i % kCols, at = row < before ? t_begin + row : after + row - before;
+            const long long n = (long long)(before + t_end - after) * kCols;  // 2^25 padded tokens pass 31 bits
+            for (long long i = tid; i < n; i += kThreads) {
+                const int row = (int)(i / kCols), col = (int)(i % kCols), at = row < before ? t_begin + row : after + row - before;
                 if (col >= cols) continue;
                 char* q = o + ((long long)(rev ? c.seqlen - 1 - at : at) * r.o.st + col * r.o.sd) * eb;
                 if (r.out_f32)

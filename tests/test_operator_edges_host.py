@@ -1,0 +1,32 @@
+"""Refusals at the edges of what the operators accept, through Python and the C ABI.  Nothing is launched; runs without a
+GPU."""
+import ctypes as C
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import viby_model_b200 as V
+from test_linear_attention_host import qkv
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require grad and has a data pointer: its tangent would be dropped without a word."""
+    q, k, v = qkv()
+    g, state, dout = torch.zeros(2), torch.zeros(1, 2, 8, 8), torch.zeros(1, 4, 2, 8)
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        t = [x[:, 0] for x in (q, k, v)]
+        for call in (lambda: V.linear_attention_fn(dual(q), k, v, g), lambda: V.linear_attention_fn(q, dual(k), v, g),
+                     lambda: V.linear_attention_fn(q, k, dual(v), g), lambda: V.linear_attention_fn(q, k, v, dual(g)),
+                     lambda: V.linear_attention_fn(q, k, v, g, None, dual(state), True),
+                     lambda: V.linear_attention_fn(q, k, v, g, out=dual(dout)),
+                     lambda: V.linear_attention_bwd(q, k, v, g, dual(dout)),
+                     lambda: V.linear_attention_bwd(q, k, v, g, dout, None, state, dual(state)),
+                     lambda: V.linear_attention_update(dual(t[0]), t[1], t[2], state, g),
+                     lambda: V.linear_attention_update(*t, dual(state), g),
+                     lambda: V.PageTable([state, dual(state)]), lambda: V.reorder_pages([dual(state)], torch.tensor([0]))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="CUDA device"):  # inputs without tangents: as ever
+            V.linear_attention_fn(q, k, v, g)

@@ -19,7 +19,7 @@ from typing import Iterable, Tuple
 import torch
 
 from . import _cabi
-from .ops import _stream_handle
+from .ops import _no_tangents, _stream_handle
 
 _nbytes, _requires_grad = attrgetter("nbytes"), attrgetter("requires_grad")
 _INDEX_DTYPES = {torch.int32: _cabi.VC1D_I32, torch.int64: _cabi.VC1D_I64}
@@ -45,6 +45,7 @@ class PageTable:
 
     def __init__(self, states: Iterable[torch.Tensor]):
         self.states = list(states)
+        _no_tangents("moving pages", *self.states)
         self.device = self.states[0].device if self.states else None
         self.pages = int(self.states[0].shape[0]) if self.states and self.states[0].dim() else 0
         # three numbers a tensor: address, bytes of a page, bytes from page to page.  A model's cache has many small

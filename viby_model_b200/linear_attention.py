@@ -14,7 +14,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _cabi
-from .ops import _IO_DTYPES, _MASK_DTYPES, _TLS, _require_cuda, _stream_handle
+from .ops import _IO_DTYPES, _MASK_DTYPES, _TLS, _no_tangents, _require_cuda, _stream_handle
 
 
 def _launch(device: torch.device, call, *args):
@@ -268,7 +268,8 @@ def linear_attention_fn(
       scale: a number, ``dim_k ** -0.5`` by default.
       kernel: None, "simt", "mma" or "tc"; segments: parts of the time axis (0 = automatic), for benches and tests.
 
-    Differentiable in q, k, v and initial_states, through o and the final state (``linear_attention_bwd``).
+    Differentiable in q, k, v and initial_states, through o and the final state (``linear_attention_bwd``); in reverse mode
+    only, inputs with a tangent are refused.
     """
     _check_scale(scale)
     if torch.is_grad_enabled() and log_decay.requires_grad:
@@ -280,6 +281,7 @@ def linear_attention_fn(
                                                    float(q.shape[-1] ** -0.5 if scale is None else scale),
                                                    bool(return_final_states))
         return (o, state) if return_final_states else o
+    _no_tangents("linear_attention_fn", q, k, v, log_decay, initial_states, out, final_states_out)
     needs_grad = torch.is_grad_enabled() and (
         q.requires_grad or k.requires_grad or v.requires_grad
         or (initial_states is not None and initial_states.requires_grad)
@@ -316,6 +318,7 @@ def linear_attention_bwd(
     where the final state was used, ``dfinal_states`` of that.  ``dinitial`` (fp32) is None unless ``need_dinitial``
     (default: when ``initial_states`` is given).  Gradients of shared key / value heads are summed over their heads."""
     _check_scale(scale)
+    _no_tangents("linear_attention_bwd", q, k, v, log_decay, dout, initial_states, dfinal_states)
     if need_dinitial is None:
         need_dinitial = initial_states is not None
     if seq_idx is not None and (attention_mask is not None or initial_states is not None or dfinal_states is not None or need_dinitial):
@@ -414,6 +417,7 @@ def _update(q, k, v, state, log_decay, attention_mask, scale, out):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
                                     or log_decay.requires_grad):
         raise ValueError("linear_attention_update has no gradient: use linear_attention_fn with seqlen 1 and initial_states")
+    _no_tangents("linear_attention_update", q, k, v, state, log_decay, out)
     key = None
     if out is None and q.is_cuda and log_decay.is_contiguous():
         key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype,

@@ -16,6 +16,7 @@ import threading
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 
@@ -46,6 +47,14 @@ def _activation_code(activation) -> int:
 def _require_cuda(t: torch.Tensor, what: str) -> None:
     if t.device.type != "cuda":
         raise ValueError(f"{what} tensor must be on a CUDA device, got {t.device}")
+
+
+def _no_tangents(what: str, *tensors) -> None:
+    """Refuses dual tensors of ``torch.autograd.forward_ad``: they have a data pointer like any other and do not require
+    grad, so a kernel would run on them and their tangents would be lost."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative, and an input has a tangent")
 
 
 def _check_weight_shapes(weight: torch.Tensor, bias: Optional[torch.Tensor], dim: int) -> int:

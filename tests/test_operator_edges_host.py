@@ -30,3 +30,17 @@ def test_forward_mode_derivatives_are_refused():
                 call()
         with pytest.raises(ValueError, match="CUDA device"):  # inputs without tangents: as ever
             V.linear_attention_fn(q, k, v, g)
+
+
+def test_forward_mode_derivatives_of_the_convolution_are_refused():
+    x, w, b, state = torch.zeros(2, 8, 5), torch.zeros(8, 4), torch.zeros(8), torch.zeros(2, 8, 4)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: V.causal_conv1d_fn(dual(x), w, b), lambda: V.causal_conv1d_fn(x, dual(w), b),
+                     lambda: V.causal_conv1d_fn(x, w, b, residual=dual(x)), lambda: V.causal_conv1d_bwd(x, w, b, dual(x)),
+                     lambda: V.causal_conv1d_update(dual(x[:, :, 0]), state, w, b),
+                     lambda: V.causal_conv1d_update(x[:, :, 0], dual(state), w, b),
+                     lambda: V.causal_conv1d_update_bwd(x[:, :, 0], state, w, b, dual(x[:, :, 0])),
+                     lambda: V.causal_conv1d_update_multi([x[:, :, 0]], [dual(state)], [w], [b])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

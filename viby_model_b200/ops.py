@@ -203,6 +203,7 @@ def causal_conv1d_fn(
             initial_states, _activation_code(activation), residual is True, bool(skip_masked_loads),
             L if want_state else 0)
         return (y, state) if want_state else y
+    _no_tangents("causal_conv1d_fn", x, weight, bias, residual, initial_states, out, final_states_out)
     needs_grad = torch.is_grad_enabled() and (
         x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
         or (isinstance(residual, torch.Tensor) and residual.requires_grad)
@@ -554,6 +555,7 @@ def causal_conv1d_bwd(
     kernel (stages, ctas_per_sm, variant).  ``seq_idx[batch, seqlen]`` (int32): the forward ran on packed
     rows; gradients stay inside each run of equal ids (no mask, no initial state).
     """
+    _no_tangents("causal_conv1d_bwd", x, weight, bias, dy, initial_states)
     if x.dim() != 3:
         raise ValueError(f"Expected 3D input tensor (batch, dim, seqlen), got {x.dim()}D")
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
@@ -780,6 +782,7 @@ def causal_conv1d_update(
             y = torch.ops.vc1d.update(x2, conv_state, weight, bias, cache_seqlens, _activation_code(activation),
                                       bool(residual))
         return y.unsqueeze(-1) if squeeze else y
+    _no_tangents("causal_conv1d_update", x, conv_state, weight, bias, out)
     needs_grad = torch.is_grad_enabled() and (
         x.requires_grad or weight.requires_grad or conv_state.requires_grad
         or (bias is not None and bias.requires_grad)
@@ -809,6 +812,7 @@ class UpdateTable:
         n = len(xs)
         if not (len(conv_states) == n and len(weights) == n):
             raise ValueError("xs, conv_states and weights must have the same length")
+        _no_tangents("a table of decode steps", *xs, *conv_states, *weights, *(biases or ()), *(outs or ()))
         biases = [None] * n if biases is None else biases
         cache_seqlens = [None] * n if cache_seqlens is None else cache_seqlens
         outs = [None] * n if outs is None else outs
@@ -886,6 +890,7 @@ def causal_conv1d_update_bwd(
     """Gradients of one decode step: ``(dx, dstate, dweight, dbias)`` for ``x[batch, dim]``,
     ``conv_state[batch, dim, state_len]`` AS IT WAS BEFORE the step, and the upstream ``dy[batch, dim]``.
     ``dweight`` / ``dbias`` are fp32 sums (causal-conv1d-mps causal_conv1d.metal:1738-1845)."""
+    _no_tangents("causal_conv1d_update_bwd", x, conv_state, weight, bias, dy)
     if x.dim() != 2 or conv_state.dim() != 3:
         raise ValueError("expected x [batch, dim] and conv_state [batch, dim, state_len]")
     batch, dim = x.shape

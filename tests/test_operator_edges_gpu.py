@@ -31,3 +31,31 @@ def test_padding_of_more_than_2_to_the_25_tokens(side):
     check(state, ref_s, tolerance(ref_s, M_s, torch.bfloat16, D, n, True, torch.float32), "state")
     out[:, at] = 0
     assert not bool(out.view(torch.int32).any())  # +0, every one of them
+
+
+@pytest.mark.parametrize("kernel", ["simt", "mma", "tc"])
+def test_the_named_kernel_runs_under_compile_too(kernel):
+    """Forward and backward; each kernel rounds differently, so that equal bits show which one ran."""
+    q, k, v, do, s0, ds = (x.to(DEV) for x in make(1, 260, 2, 1, 2, 64, 64, torch.bfloat16))
+    g = decays(2).to(DEV)
+
+    def f(q, k, v, s0):
+        return V.linear_attention_fn(q, k, v, g, None, s0, True, kernel=kernel, segments=2)
+
+    torch._dynamo.reset()
+    results = []
+    for call in (f, torch.compile(f, fullgraph=True)):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v, s0)]
+        o, s = call(*leaves)
+        before = V.last_kernel()
+        results.append((o, s, *torch.autograd.grad([o, s], leaves, [do, ds])))
+        assert before == f"linear_{kernel}"
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_an_unknown_kernel_is_refused_under_compile():
+    q, k, v, *_ = (x.to(DEV) for x in make(1, 8, 2, 2, 2, 16, 16, torch.bfloat16))
+    g = decays(2).to(DEV)
+    with pytest.raises(Exception, match="unknown linear attention kernel"):
+        torch.compile(lambda q: V.linear_attention_fn(q, k, v, g, kernel="best"))(q)

@@ -149,14 +149,15 @@ torch.library.register_autograd("vc1d::update_fn", _update_backward, setup_conte
 @torch.library.custom_op("vc1d::linear_attention", mutates_args=(), device_types="cuda")
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, seq_idx: Optional[torch.Tensor],
                      initial_states: Optional[torch.Tensor], mask: Optional[torch.Tensor], scale: float,
-                     want_state: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """o (and, with want_state, the final state) of linear_attention_fn."""
-    o, state = la._forward(q, k, v, log_decay, seq_idx, initial_states, want_state, None, mask, scale, None, None, 0)
+                     want_state: bool, kernel_name: str = "auto", segments: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """o (and, with want_state, the final state) of linear_attention_fn.  (Inductor passes an argument called ``kernel`` of its
+    own, hence ``kernel_name``.)"""
+    o, state = la._forward(q, k, v, log_decay, seq_idx, initial_states, want_state, None, mask, scale, None, kernel_name, segments)
     return o, state if state is not None else q.new_empty(0, dtype=torch.float32)
 
 
 @linear_attention.register_fake
-def _(q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state):
+def _(q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state, kernel_name="auto", segments=0):
     o = q.new_empty((q.shape[0], q.shape[1], q.shape[2], v.shape[3]))
     shape = (q.shape[0], q.shape[2], q.shape[3], v.shape[3]) if want_state else (0,)
     return o, q.new_empty(shape, dtype=torch.float32)
@@ -165,31 +166,32 @@ def _(q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state):
 @torch.library.custom_op("vc1d::linear_attention_bwd", mutates_args=(), device_types="cuda")
 def linear_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, dout: torch.Tensor,
                          seq_idx: Optional[torch.Tensor], initial_states: Optional[torch.Tensor],
-                         dfinal_states: Optional[torch.Tensor], mask: Optional[torch.Tensor], scale: float
+                         dfinal_states: Optional[torch.Tensor], mask: Optional[torch.Tensor], scale: float,
+                         kernel_name: str = "auto", segments: int = 0
                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     dq, dk, dv, dinit = la.linear_attention_bwd(q, k, v, log_decay, dout, seq_idx, initial_states, dfinal_states,
-                                                attention_mask=mask, scale=scale)
+                                                attention_mask=mask, scale=scale, kernel=kernel_name, segments=segments)
     return dq, dk, dv, dinit if dinit is not None else q.new_empty(0, dtype=torch.float32)
 
 
 @linear_attention_bwd.register_fake
-def _(q, k, v, log_decay, dout, seq_idx, initial_states, dfinal_states, mask, scale):
+def _(q, k, v, log_decay, dout, seq_idx, initial_states, dfinal_states, mask, scale, kernel_name="auto", segments=0):
     dinit = q.new_empty(initial_states.shape if initial_states is not None else (0,), dtype=torch.float32)
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), dinit
 
 
 def _linear_setup(ctx, inputs, output):
-    q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state = inputs
+    q, k, v, log_decay, seq_idx, initial_states, mask, scale, want_state, kernel_name, segments = inputs
     ctx.save_for_backward(q, k, v, log_decay, seq_idx, initial_states, mask)
-    ctx.scale = scale
+    ctx.scale, ctx.kernel, ctx.segments = scale, kernel_name, segments
     ctx.want_state = want_state
 
 
 def _linear_backward(ctx, dout, dstate):
     q, k, v, log_decay, seq_idx, init, mask = ctx.saved_tensors
     dq, dk, dv, dinit = torch.ops.vc1d.linear_attention_bwd(q, k, v, log_decay, dout, seq_idx, init,
-                                                            dstate if ctx.want_state else None, mask, ctx.scale)
-    return dq, dk, dv, None, None, dinit if init is not None else None, None, None, None
+                                                            dstate if ctx.want_state else None, mask, ctx.scale, ctx.kernel, ctx.segments)
+    return dq, dk, dv, None, None, dinit if init is not None else None, None, None, None, None, None
 
 
 torch.library.register_autograd("vc1d::linear_attention", _linear_backward, setup_context=_linear_setup)

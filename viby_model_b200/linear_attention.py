@@ -266,7 +266,9 @@ def linear_attention_fn(
       attention_mask ``[batch, seqlen]`` (bool / int / float; nonzero = valid): a masked token is not read, leaves the state
         as it is (no decay either) and its output is 0.
       scale: a number, ``dim_k ** -0.5`` by default.
-      kernel: None, "simt", "mma" or "tc"; segments: parts of the time axis (0 = automatic), for benches and tests.
+      kernel: None, "simt", "mma" or "tc".  16-bit inputs go to the tensor cores by default, where the products inside a chunk
+        and the state that queries read are rounded to 16 bits before the second product; "simt" keeps both in fp32, at the
+        fp32 pipes' speed.  segments: parts of the time axis (0 = automatic).
 
     Differentiable in q, k, v and initial_states, through o and the final state (``linear_attention_bwd``); in reverse mode
     only, inputs with a tangent are refused.
@@ -279,7 +281,7 @@ def linear_attention_fn(
             raise ValueError("out= / final_states_out= cannot be used under torch.compile")
         o, state = torch.ops.vc1d.linear_attention(q, k, v, log_decay, seq_idx, initial_states, attention_mask,
                                                    float(q.shape[-1] ** -0.5 if scale is None else scale),
-                                                   bool(return_final_states))
+                                                   bool(return_final_states), kernel or "auto", int(segments))
         return (o, state) if return_final_states else o
     _no_tangents("linear_attention_fn", q, k, v, log_decay, initial_states, out, final_states_out)
     needs_grad = torch.is_grad_enabled() and (

@@ -59,3 +59,21 @@ def test_an_unknown_kernel_is_refused_under_compile():
     g = decays(2).to(DEV)
     with pytest.raises(Exception, match="unknown linear attention kernel"):
         torch.compile(lambda q: V.linear_attention_fn(q, k, v, g, kernel="best"))(q)
+
+
+@pytest.mark.parametrize("kernel", [None, "simt", "mma", "tc"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [16, 160, 256])
+def test_calls_without_tokens_copy_the_state(dtype, D, kernel):
+    """There is nothing to make tensor maps of, so none of the kernels that take tokens by them may run."""
+    q, k, v, do, s0, ds = (x.to(DEV) for x in make(2, 0, 2, 1, 2, D, D, dtype))
+    g = decays(2).to(DEV)
+    for initial in (s0, None):
+        o, s = V.linear_attention_fn(q, k, v, g, None, initial, True, kernel=kernel, segments=2)
+        assert V.last_kernel() == "linear_simt"
+        assert tuple(o.shape) == (2, 0, 2, D) and torch.equal(s, s0 if initial is not None else torch.zeros_like(s0))
+    for dfinal in (ds, None):
+        *grads, di = V.linear_attention_bwd(q, k, v, g, do, None, s0, dfinal, kernel=kernel)
+        assert V.last_kernel() == "linear_simt"
+        assert all(x.shape == y.shape for x, y in zip(grads, (q, k, v)))
+        assert torch.equal(di, ds if dfinal is not None else torch.zeros_like(ds))

@@ -199,6 +199,7 @@ bool tma_fits(const Launch& l) {
     return true;
 }
 Kind pick(const Launch& l, int dtype, int kernel) {
+    if (l.c.seqlen == 0) return kSimt;  // copies the state; there is nothing to make tensor maps of
     if (kernel == VC1D_LINEAR_SIMT || !mma_fits(l, dtype)) return kSimt;
     return kernel != VC1D_LINEAR_MMA && dtype == VC1D_BF16 && largest_rows(l) <= 160 && tma_fits(l) ? kTc : kMma;
 }

@@ -843,8 +843,8 @@ cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) 
         }
         slabs = max(slabs, (r.dv + kCols - 1) / kCols);
         Maps& m = maps.run[i];
-        if (l.c.seqlen > 0 && !(encode(&m.a, r.a, l.c.batch, l.c.heads, l.c.seqlen, r.da) && encode(&m.k, r.k, l.c.batch, l.c.heads, l.c.seqlen, r.da) &&
-                                encode(&m.v, r.v, l.c.batch, l.c.heads, l.c.seqlen, r.dv)))
+        if (!(encode(&m.a, r.a, l.c.batch, l.c.heads, l.c.seqlen, r.da) && encode(&m.k, r.k, l.c.batch, l.c.heads, l.c.seqlen, r.da) &&
+              encode(&m.v, r.v, l.c.batch, l.c.heads, l.c.seqlen, r.dv)))
             return cudaErrorNotSupported;
     }
     auto kernel = k_linear_tc<ROWS, STATES, REV>;

@@ -1,12 +1,15 @@
 """Refusals at the edges of what the operators accept, through Python and the C ABI.  Nothing is launched; runs without a
 GPU."""
-import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import viby_model_b200 as V
+from conftest import ROOT
 from test_linear_attention_host import qkv
 
 
@@ -44,3 +47,14 @@ def test_forward_mode_derivatives_of_the_convolution_are_refused():
                      lambda: V.causal_conv1d_update_multi([x[:, :, 0]], [dual(state)], [w], [b])):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def test_one_page_of_overlapping_tensors_without_a_stride():
+    """Strides say nothing where there is one page.  In a process of its own: a division by such a stride ends it."""
+    code = ("import ctypes as C, sys; sys.path[:0] = ['tests', '.']\n"
+            "from test_linear_attention_host import FAKE, page_args\n"
+            "from viby_model_b200 import _cabi\n"
+            "for tensors in ([(FAKE, 16, 0), (FAKE, 16, 0)], [(FAKE, 16, 0), (FAKE + 8, 16, 0)], [(FAKE, 16, -4), (FAKE, 16, -4)]):\n"
+            "    assert _cabi.lib.vc1d_pages(C.byref(page_args(tensors, pages=1)), None) == _cabi.VC1D_E_ALIAS\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, env=dict(os.environ))
+    assert r.returncode == 0, (r.returncode, r.stderr[-2000:])

@@ -227,7 +227,7 @@ bool overlap(const vc1d_page_tensor& a, const vc1d_page_tensor& b, int pages) {
     const char *a0 = static_cast<const char*>(a.base), *b0 = static_cast<const char*>(b.base);
     const char *a1 = a0 + (pages - 1) * a.stride_bytes + a.page_bytes, *b1 = b0 + (pages - 1) * b.stride_bytes + b.page_bytes;
     if (a1 <= b0 || b1 <= a0) return false;
-    if (a.stride_bytes != b.stride_bytes) return true;
+    if (pages == 1 || a.stride_bytes != b.stride_bytes) return true;  // one page: any stride is allowed, 0 too
     const long long s = a.stride_bytes, d = (((b0 - a0) % s) + s) % s;  // b's pages start d bytes after a's, modulo the stride
     return d < a.page_bytes || d + b.page_bytes > s;
 }

@@ -1,5 +1,6 @@
 """Refusals at the edges of what the operators accept, through Python and the C ABI.  Nothing is launched; runs without a
 GPU."""
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -10,7 +11,8 @@ from torch.autograd import forward_ad
 
 import viby_model_b200 as V
 from conftest import ROOT
-from test_linear_attention_host import qkv
+from test_linear_attention_host import FAKE, POINTERS, linear_args, qkv
+from viby_model_b200 import _cabi
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -58,3 +60,54 @@ def test_one_page_of_overlapping_tensors_without_a_stride():
             "    assert _cabi.lib.vc1d_pages(C.byref(page_args(tensors, pages=1)), None) == _cabi.VC1D_E_ALIAS\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, env=dict(os.environ))
     assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
+
+
+F32_STATES = dict(initial_strides=(128, 64, 8, 1), final_strides=(128, 64, 8, 1))
+SIDES = [dict(mask=4 * FAKE + 16, mask_dtype=_cabi.VC1D_U8, mask_strides=(4, 1)),
+         dict(mask=4 * FAKE - 24, mask_dtype=_cabi.VC1D_I64, mask_strides=(4, 1)),
+         dict(seq_idx=4 * FAKE + 8, seq_strides=(4, 1)), dict(log_decay=4 * FAKE + 4), dict(log_decay=4 * FAKE - 4)]
+
+
+@pytest.mark.parametrize("side", SIDES)
+def test_outputs_over_masks_sequence_numbers_and_decays_are_refused(side):
+    """Some CTAs would read them while others already store."""
+    before = _cabi.launch_count()
+    a = linear_args(**{**POINTERS, **side})  # out lies at 4 * FAKE
+    assert _cabi.lib.vc1d_linear(C.byref(a), None) == _cabi.VC1D_E_ALIAS
+    if "seq_idx" not in side:  # states and packed rows are not combined
+        a = linear_args(**{**POINTERS, **side, "out": 6 * FAKE, "final_state": 4 * FAKE, **F32_STATES})
+        assert _cabi.lib.vc1d_linear(C.byref(a), None) == _cabi.VC1D_E_ALIAS
+        a = linear_args(**{**POINTERS, "seqlen": 0, "log_decay": 4 * FAKE, "final_state": 4 * FAKE, **F32_STATES})
+        assert _cabi.lib.vc1d_linear(C.byref(a), None) == _cabi.VC1D_E_ALIAS
+    for grad in ("dq", "dk", "dv", "dinitial"):
+        if grad == "dinitial" and "seq_idx" in side:
+            continue
+        b = _cabi.LinearBwdArgs()
+        b.struct_size = C.sizeof(_cabi.LinearBwdArgs)
+        b.f = linear_args(**{**POINTERS, **side, "out": None})
+        b.dout, b.dq, b.dk, b.dv = 8 * FAKE, 9 * FAKE, 10 * FAKE, 11 * FAKE
+        for name in ("dout", "dq", "dk", "dv"):
+            getattr(b, name + "_strides")[:] = (64, 16, 8, 1)
+        b.dinitial_strides[:] = (128, 64, 8, 1)
+        setattr(b, grad, 4 * FAKE)
+        assert _cabi.lib.vc1d_linear_bwd(C.byref(b), None) == _cabi.VC1D_E_ALIAS, grad
+    assert _cabi.launch_count() == before
+
+
+@pytest.mark.parametrize("written", ["out", "state"])
+@pytest.mark.parametrize("side", [dict(mask=4 * FAKE + 1, mask_dtype=_cabi.VC1D_U8, mask_stride=1),
+                                  dict(mask=4 * FAKE - 8, mask_dtype=_cabi.VC1D_F32, mask_stride=2), dict(log_decay=4 * FAKE + 4)])
+def test_a_token_written_over_its_mask_or_decays_is_refused(side, written):
+    a = _cabi.LinearUpdateArgs()
+    a.struct_size = C.sizeof(_cabi.LinearUpdateArgs)
+    a.dtype = _cabi.VC1D_F16
+    a.batch, a.heads, a.heads_k, a.heads_v, a.dim_k, a.dim_v = 2, 2, 1, 2, 8, 8
+    a.q, a.k, a.v, a.out, a.state, a.log_decay = FAKE, 2 * FAKE, 3 * FAKE, 5 * FAKE, 6 * FAKE, 7 * FAKE
+    a.q_strides[:], a.k_strides[:], a.v_strides[:], a.out_strides[:] = (16, 8, 1), (8, 8, 1), (16, 8, 1), (16, 8, 1)
+    a.state_strides[:] = (128, 64, 8, 1)
+    setattr(a, written, 4 * FAKE)
+    for k, v in side.items():
+        setattr(a, k, v)
+    before = _cabi.launch_count()
+    assert _cabi.lib.vc1d_linear_update(C.byref(a), None) == _cabi.VC1D_E_ALIAS
+    assert _cabi.launch_count() == before

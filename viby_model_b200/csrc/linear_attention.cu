@@ -107,31 +107,40 @@ int check(const vc1d_linear_args* a) {
     return VC1D_OK;
 }
 
+// What every pass reads: the decays, the initial state, and with tokens q, k, v, the mask and the sequence numbers.
+Touched inputs(const vc1d_linear_args& a) {
+    const Shape n = shape_of(a);
+    const int eb = elem_bytes(a.dtype), n_bt[2] = {a.batch, a.seqlen}, n_h[1] = {a.heads};
+    const int64_t one[1] = {1};
+    Touched t;
+    t.reads_from(extent(a.log_decay, 4, n_h, one));
+    if (a.initial_state != nullptr) t.reads_from(extent(a.initial_state, 4, n.s, a.initial_strides));
+    if (a.seqlen == 0) return t;
+    t.reads_from(extent(a.q, eb, n.q, a.q_strides));
+    t.reads_from(extent(a.k, eb, n.k, a.k_strides));
+    t.reads_from(extent(a.v, eb, n.v, a.v_strides));
+    if (a.mask != nullptr) t.reads_from(extent(a.mask, elem_bytes(a.mask_dtype), n_bt, a.mask_strides));
+    if (a.seq_idx != nullptr) t.reads_from(extent(a.seq_idx, 4, n_bt, a.seq_strides));
+    return t;
+}
+
 int check_forward(const vc1d_linear_args* a) {
     const int st = check(a);
     if (st != VC1D_OK) return st;
     if (a->batch == 0) return VC1D_OK;
     if (a->log_decay == nullptr) return VC1D_E_NULL;
     const Shape n = shape_of(*a);
-    const int eb = elem_bytes(a->dtype);
+    Touched t = inputs(*a);
     if (a->seqlen > 0) {
         if (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->out == nullptr) return VC1D_E_NULL;
         if (!writable(n.o, a->out_strides)) return VC1D_E_STRIDE;
-        const Range o = extent(a->out, eb, n.o, a->out_strides);
-        if (overlap(o, extent(a->q, eb, n.q, a->q_strides)) || overlap(o, extent(a->k, eb, n.k, a->k_strides)) ||
-            overlap(o, extent(a->v, eb, n.v, a->v_strides)) ||
-            (a->initial_state != nullptr && overlap(o, extent(a->initial_state, 4, n.s, a->initial_strides))))
-            return VC1D_E_ALIAS;
+        t.writes_to(extent(a->out, elem_bytes(a->dtype), n.o, a->out_strides));
     }
     if (a->final_state != nullptr) {
         if (!writable(n.s, a->final_strides)) return VC1D_E_STRIDE;
-        const Range f = extent(a->final_state, 4, n.s, a->final_strides);
-        if (a->initial_state != nullptr && overlap(f, extent(a->initial_state, 4, n.s, a->initial_strides))) return VC1D_E_ALIAS;
-        if (a->seqlen > 0 && (overlap(f, extent(a->out, eb, n.o, a->out_strides)) || overlap(f, extent(a->q, eb, n.q, a->q_strides)) ||
-                              overlap(f, extent(a->k, eb, n.k, a->k_strides)) || overlap(f, extent(a->v, eb, n.v, a->v_strides))))
-            return VC1D_E_ALIAS;
+        t.writes_to(extent(a->final_state, 4, n.s, a->final_strides));
     }
-    return VC1D_OK;
+    return t.clash() ? VC1D_E_ALIAS : VC1D_OK;
 }
 
 Rows rows(const void* p, const int64_t (&s)[4], int group) { return {p, s[0], s[1], s[2], s[3], group}; }
@@ -299,32 +308,22 @@ int check_backward(const vc1d_linear_bwd_args* a) {
     if (f.log_decay == nullptr) return VC1D_E_NULL;
     const Shape n = shape_of(f);
     const int eb = elem_bytes(f.dtype);
+    Touched t = inputs(f);
+    if (a->dfinal != nullptr) t.reads_from(extent(a->dfinal, 4, n.s, a->dfinal_strides));
     if (f.seqlen > 0) {
         if (f.q == nullptr || f.k == nullptr || f.v == nullptr || a->dout == nullptr || a->dq == nullptr || a->dk == nullptr || a->dv == nullptr)
             return VC1D_E_NULL;
         if (!writable(n.q, a->dq_strides) || !writable(n.k, a->dk_strides) || !writable(n.v, a->dv_strides)) return VC1D_E_STRIDE;
-        const Range in[4] = {extent(f.q, eb, n.q, f.q_strides), extent(f.k, eb, n.k, f.k_strides), extent(f.v, eb, n.v, f.v_strides),
-                             extent(a->dout, eb, n.o, a->dout_strides)};
-        const Range out[3] = {extent(a->dq, eb, n.q, a->dq_strides), extent(a->dk, eb, n.k, a->dk_strides), extent(a->dv, eb, n.v, a->dv_strides)};
-        for (const Range& o : out) {
-            for (const Range& i : in)
-                if (overlap(o, i)) return VC1D_E_ALIAS;
-            if (f.initial_state != nullptr && overlap(o, extent(f.initial_state, 4, n.s, f.initial_strides))) return VC1D_E_ALIAS;
-            if (a->dfinal != nullptr && overlap(o, extent(a->dfinal, 4, n.s, a->dfinal_strides))) return VC1D_E_ALIAS;
-            if (a->dinitial != nullptr && overlap(o, extent(a->dinitial, 4, n.s, a->dinitial_strides))) return VC1D_E_ALIAS;
-        }
-        if (a->dinitial != nullptr)
-            for (const Range& i : in)
-                if (overlap(i, extent(a->dinitial, 4, n.s, a->dinitial_strides))) return VC1D_E_ALIAS;
-        if (overlap(out[0], out[1]) || overlap(out[0], out[2]) || overlap(out[1], out[2])) return VC1D_E_ALIAS;
+        t.reads_from(extent(a->dout, eb, n.o, a->dout_strides));
+        t.writes_to(extent(a->dq, eb, n.q, a->dq_strides));
+        t.writes_to(extent(a->dk, eb, n.k, a->dk_strides));
+        t.writes_to(extent(a->dv, eb, n.v, a->dv_strides));
     }
     if (a->dinitial != nullptr) {
         if (!writable(n.s, a->dinitial_strides)) return VC1D_E_STRIDE;
-        const Range d = extent(a->dinitial, 4, n.s, a->dinitial_strides);
-        if (a->dfinal != nullptr && overlap(d, extent(a->dfinal, 4, n.s, a->dfinal_strides))) return VC1D_E_ALIAS;
-        if (f.initial_state != nullptr && overlap(d, extent(f.initial_state, 4, n.s, f.initial_strides))) return VC1D_E_ALIAS;
+        t.writes_to(extent(a->dinitial, 4, n.s, a->dinitial_strides));
     }
-    return VC1D_OK;
+    return t.clash() ? VC1D_E_ALIAS : VC1D_OK;
 }
 
 // dq: tokens in order.  Then dk and dv: tokens from the last to the first.

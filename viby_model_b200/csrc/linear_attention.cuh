@@ -150,6 +150,23 @@ Range extent(const void* base, int eb, const int (&n)[D], const int64_t (&s)[D])
     return {b + lo * eb, b + (hi + 1) * eb};
 }
 inline bool overlap(const Range& a, const Range& b) { return a.lo < b.hi && b.lo < a.hi; }
+// Memory that a call reads and memory that it writes: what is written may overlap nothing else, the decays, masks and
+// sequence numbers included, because some CTAs read them while others already store.
+struct Touched {
+    Range read[12], written[4];
+    int reads = 0, writes = 0;
+    void reads_from(const Range& r) { read[reads++] = r; }
+    void writes_to(const Range& r) { written[writes++] = r; }
+    bool clash() const {
+        for (int i = 0; i < writes; ++i) {
+            for (int j = 0; j < reads; ++j)
+                if (overlap(written[i], read[j])) return true;
+            for (int j = 0; j < i; ++j)
+                if (overlap(written[i], written[j])) return true;
+        }
+        return false;
+    }
+};
 // a written tensor gives every element a place of its own: no stride 0 along an axis of more than one entry
 template <int D>
 bool writable(const int (&n)[D], const int64_t (&s)[D]) {

@@ -161,13 +161,17 @@ VC1D_API int vc1d_linear_update(const vc1d_linear_update_args* a, void* stream) 
     const int n_q[3] = {a->batch, a->heads, a->dim_k}, n_k[3] = {a->batch, a->heads_k, a->dim_k}, n_v[3] = {a->batch, a->heads_v, a->dim_v},
               n_o[3] = {a->batch, a->heads, a->dim_v}, n_s[4] = {a->batch, a->heads, a->dim_k, a->dim_v};
     if (!lin::writable(n_o, a->out_strides) || !lin::writable(n_s, a->state_strides)) return VC1D_E_STRIDE;
-    const int eb = elem_bytes(a->dtype);
-    const lin::Range in[3] = {lin::extent(a->q, eb, n_q, a->q_strides), lin::extent(a->k, eb, n_k, a->k_strides),
-                              lin::extent(a->v, eb, n_v, a->v_strides)};
-    const lin::Range o = lin::extent(a->out, eb, n_o, a->out_strides), st = lin::extent(a->state, 4, n_s, a->state_strides);
-    if (lin::overlap(o, st)) return VC1D_E_ALIAS;
-    for (const lin::Range& r : in)
-        if (lin::overlap(o, r) || lin::overlap(st, r)) return VC1D_E_ALIAS;
+    const int eb = elem_bytes(a->dtype), n_h[1] = {a->heads}, n_b[1] = {a->batch};
+    const int64_t one[1] = {1}, mask_stride[1] = {a->mask_stride};
+    lin::Touched t;
+    t.reads_from(lin::extent(a->q, eb, n_q, a->q_strides));
+    t.reads_from(lin::extent(a->k, eb, n_k, a->k_strides));
+    t.reads_from(lin::extent(a->v, eb, n_v, a->v_strides));
+    t.reads_from(lin::extent(a->log_decay, 4, n_h, one));
+    if (a->mask != nullptr) t.reads_from(lin::extent(a->mask, elem_bytes(a->mask_dtype), n_b, mask_stride));
+    t.writes_to(lin::extent(a->out, eb, n_o, a->out_strides));
+    t.writes_to(lin::extent(a->state, 4, n_s, a->state_strides));
+    if (t.clash()) return VC1D_E_ALIAS;
     LUParams p{};
     p.q = a->q;
     p.k = a->k;

@@ -440,7 +440,8 @@ VC1D_API uint32_t vc1d_sizeof_linear_update_args(void);
  *   VC1D_PAGES_FREE:    dst[n]: page dst[i] is cleared to zero bytes
  *   VC1D_PAGES_COMPACT: live[pages] (bytes, 0 = free): with n = number of live pages, the free pages below n take,
  *                       in order, the live pages from n on; pages from n on are left as they are.  new_index[pages]
- *                       receives where each page is afterwards (-1: it was free), count[1] receives n.
+ *                       receives where each page is afterwards (-1: it was free), count[1] receives n. The three
+ *                       arrays do not overlap.
  * A source or destination outside 0..pages-1 moves nothing (checked by the kernel).
  */
 #define VC1D_PAGES_MAX_TENSORS 128

@@ -11,7 +11,7 @@ from torch.autograd import forward_ad
 
 import viby_model_b200 as V
 from conftest import ROOT
-from test_linear_attention_host import FAKE, POINTERS, linear_args, qkv
+from test_linear_attention_host import FAKE, POINTERS, linear_args, page_args, qkv
 from viby_model_b200 import _cabi
 
 
@@ -110,4 +110,16 @@ def test_a_token_written_over_its_mask_or_decays_is_refused(side, written):
         setattr(a, k, v)
     before = _cabi.launch_count()
     assert _cabi.lib.vc1d_linear_update(C.byref(a), None) == _cabi.VC1D_E_ALIAS
+    assert _cabi.launch_count() == before
+
+
+@pytest.mark.parametrize("new_index,count", [(2 * FAKE + 3, 4 * FAKE), (2 * FAKE - 12, 4 * FAKE), (3 * FAKE, 2 * FAKE), (3 * FAKE, 2 * FAKE - 1),
+                                             (3 * FAKE, 3 * FAKE + 12)])
+def test_compaction_whose_results_overlap_its_input_is_refused(new_index, count):
+    """One CTA writes them while the others still read which pages are live."""
+    before = _cabi.launch_count()
+    a = page_args([(FAKE, 64, 64)], op=_cabi.PAGES_COMPACT, live=2 * FAKE, new_index=new_index, count=count)
+    assert _cabi.lib.vc1d_pages(C.byref(a), None) == _cabi.VC1D_E_ALIAS
+    a.n_tensors = 0
+    assert _cabi.lib.vc1d_pages(C.byref(a), None) == _cabi.VC1D_E_ALIAS
     assert _cabi.launch_count() == before

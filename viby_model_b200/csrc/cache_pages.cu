@@ -232,6 +232,11 @@ bool overlap(const vc1d_page_tensor& a, const vc1d_page_tensor& b, int pages) {
     return d < a.page_bytes || d + b.page_bytes > s;
 }
 
+bool meet(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+    const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
+    return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
+}
+
 // Whether an array of the call lies among a tensor's pages: every CTA reads the index arrays while others already store.
 bool inside(const vc1d_page_tensor& t, int pages, const void* p, long long bytes) {
     if (p == nullptr || bytes == 0) return false;
@@ -259,6 +264,10 @@ VC1D_API int vc1d_pages(const vc1d_pages_args* a, void* stream) {
     if (listed && a->dst == nullptr) return VC1D_E_NULL;
     if (a->op == VC1D_PAGES_COPY && a->source == nullptr) return VC1D_E_NULL;
     if (a->n_tensors > 0 && a->tensors == nullptr) return VC1D_E_NULL;
+    // one CTA writes new_index and count while the others read live
+    if (compact && (meet(a->new_index, 4LL * a->pages, a->live, a->pages) || meet(a->count, 4, a->live, a->pages) ||
+                    meet(a->count, 4, a->new_index, 4LL * a->pages)))
+        return VC1D_E_ALIAS;
     static thread_local PParams p;
     p.n_tensors = 0;
     p.sum_page_bytes = 0;

@@ -359,7 +359,7 @@ typedef struct vc1d_linear_args {
     const void* k;          /* [batch, seqlen, heads_k, dim_k] */
     const void* v;          /* [batch, seqlen, heads_v, dim_v] */
     void* out;              /* [batch, seqlen, heads, dim_v]; what a call writes must not overlap anything else of it */
-    int64_t q_strides[4], k_strides[4], v_strides[4], out_strides[4];   /* in elements; inputs may repeat (stride 0) */
+    int64_t q_strides[4], k_strides[4], v_strides[4], out_strides[4];   /* in elements; inputs may repeat (stride 0, windows), outputs may not */
     const float* log_decay; /* [heads] */
     const void* mask;       /* [batch, seqlen] or NULL; 0 = masked */
     int64_t mask_strides[2];

@@ -123,3 +123,38 @@ def test_compaction_whose_results_overlap_its_input_is_refused(new_index, count)
     a.n_tensors = 0
     assert _cabi.lib.vc1d_pages(C.byref(a), None) == _cabi.VC1D_E_ALIAS
     assert _cabi.launch_count() == before
+
+
+OVERLAPPING = [(64, 16, 4, 1), (64, 16, 8, 2), (64, 8, 8, 1), (64, 15, 8, 1), (32, 16, 8, 1), (1, 2, 8, 1)]  # [2, 4, 2, 8]
+APART = [(64, 16, 8, 1), (64, 8, 32, 1), (8, 16, 64, 1), (64, 1, 32, 4), (1000, 17, 8, 1), (64, -16, 8, 1)]
+
+
+@pytest.mark.parametrize("strides,ok", [(s, False) for s in OVERLAPPING] + [(s, True) for s in APART])
+def test_outputs_whose_elements_share_memory_are_refused(strides, ok):
+    """Windows that overlap as well as stride 0.  Where the strides are fine, the next check (the workspace's address) refuses."""
+    places = {sum(i * s for i, s in zip((b, t, h, d), strides)) for b in range(2) for t in range(4) for h in range(2) for d in range(8)}
+    assert (len(places) == 2 * 4 * 2 * 8) == ok
+    before = _cabi.launch_count()
+    a = linear_args(**{**POINTERS, "batch": 2, "out_strides": strides, "workspace": 7 * FAKE + 4, "workspace_bytes": 1 << 20})
+    a.out = 4 * FAKE
+    want = _cabi.VC1D_E_STRIDE
+    assert _cabi.lib.vc1d_linear(C.byref(a), None) == want
+    a.mask, a.mask_dtype, a.mask_strides[:] = 4 * FAKE, _cabi.VC1D_U8, (4, 1)  # found only after the strides
+    assert _cabi.lib.vc1d_linear(C.byref(a), None) == (_cabi.VC1D_E_ALIAS if ok else want)
+    assert _cabi.launch_count() == before
+
+
+@pytest.mark.parametrize("strides,ok", [((512, 64, 8, 1), True), ((64, 128, 8, 1), True), ((512, 64, 1, 8), True), ((64, 64, 8, 1), False),
+                                        ((512, 64, 4, 1), False), ((512, 60, 8, 1), False), ((100, 64, 8, 1), False)])
+def test_states_whose_requests_share_memory_are_refused(strides, ok):
+    a = _cabi.LinearUpdateArgs()
+    a.struct_size = C.sizeof(_cabi.LinearUpdateArgs)
+    a.dtype = _cabi.VC1D_F32
+    a.batch, a.heads, a.heads_k, a.heads_v, a.dim_k, a.dim_v = 2, 2, 2, 2, 8, 8
+    a.q, a.k, a.v, a.out, a.state, a.log_decay = FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, 4 * FAKE, 7 * FAKE  # out and state overlap
+    for name in ("q", "k", "v", "out"):
+        getattr(a, name + "_strides")[:] = (16, 8, 1)
+    a.state_strides[:] = strides
+    before = _cabi.launch_count()
+    assert _cabi.lib.vc1d_linear_update(C.byref(a), None) == (_cabi.VC1D_E_ALIAS if ok else _cabi.VC1D_E_STRIDE)
+    assert _cabi.launch_count() == before

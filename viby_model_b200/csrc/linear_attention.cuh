@@ -15,6 +15,8 @@
 // as it is and the gradient of the initial state leaves as it is; the powers then shift by one (`shift` below).
 #pragma once
 
+#include <cstdlib>
+
 #include "vc1d_common.cuh"
 #include "vc1d_internal.h"
 
@@ -167,11 +169,24 @@ struct Touched {
         return false;
     }
 };
-// a written tensor gives every element a place of its own: no stride 0 along an axis of more than one entry
+// A written tensor gives every element a place of its own: each stride passes the whole extent of the axes with smaller ones
+// (no stride 0, no windows that overlap).
 template <int D>
 bool writable(const int (&n)[D], const int64_t (&s)[D]) {
-    for (int i = 0; i < D; ++i)
-        if (n[i] > 1 && s[i] == 0) return false;
+    int axis[D], used = 0;
+    for (int i = 0; i < D; ++i) {
+        if (n[i] == 0) return true;
+        if (n[i] == 1) continue;
+        int at = used++;
+        for (; at > 0 && std::llabs(s[axis[at - 1]]) > std::llabs(s[i]); --at) axis[at] = axis[at - 1];
+        axis[at] = i;
+    }
+    long long span = 0;
+    for (int i = 0; i < used; ++i) {
+        const long long stride = std::llabs(s[axis[i]]);
+        if (stride <= span) return false;
+        span += (long long)(n[axis[i]] - 1) * stride;
+    }
     return true;
 }
 

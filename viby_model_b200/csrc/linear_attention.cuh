@@ -15,6 +15,7 @@
 // as it is and the gradient of the initial state leaves as it is; the powers then shift by one (`shift` below).
 #pragma once
 
+#include <atomic>
 #include <cstdlib>
 
 #include "vc1d_common.cuh"
@@ -188,6 +189,22 @@ bool writable(const int (&n)[D], const int64_t (&s)[D]) {
         span += (long long)(n[axis[i]] - 1) * stride;
     }
     return true;
+}
+
+// Kernels whose warps have unequal shares of the registers (setmaxnreg).  A share that is raised waits, without any limit, until
+// the other warps have given up enough of what the CTA was launched with: `share` is what all warps together ask for.
+constexpr bool shares_fit(int regs_per_thread, int threads, int share) { return (regs_per_thread + 7) / 8 * 8 * threads >= share; }
+static_assert(shares_fit(80, 768, 61440) && shares_fit(73, 768, 61440) && !shares_fit(72, 768, 61440) && !shares_fit(120, 256, 32768));
+
+// Refuses a launch whose compiled kernel has not the registers that its shares add up to; asked for until it was found once.
+template <typename Kernel>
+cudaError_t check_registers(Kernel* kernel, int threads, int share, std::atomic<bool>& fits) {
+    if (fits.load(std::memory_order_relaxed)) return cudaSuccess;
+    cudaFuncAttributes at{};
+    cudaError_t e = cudaFuncGetAttributes(&at, kernel);
+    if (e == cudaSuccess && !shares_fit(at.numRegs, threads, share)) e = cudaErrorLaunchOutOfResources;
+    if (e == cudaSuccess) fits.store(true, std::memory_order_relaxed);
+    return e;
 }
 
 // The kernels.  kMma: warp-level products, 16-bit types, any head.  kTc: tcgen05, bf16, heads up to 160.

@@ -59,6 +59,7 @@ template <int DAP>
 struct Registers {
     static constexpr bool kShares = DAP <= 160 && DAP > 64;
     static constexpr int kOut = DAP == 160 ? 88 : 104, kState = 256 - kOut;
+    static constexpr int kShare = kThreads / 2 * (kOut + kState);
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -663,6 +664,11 @@ cudaError_t launch(const Launch& l, cudaStream_t s) {
     int slabs = 0;
     for (int i = 0; i < l.runs; ++i) slabs = max(slabs, (l.run[i].dv + BV - 1) / BV);
     auto kernel = k_linear_mma<DT, DAP, BV, STATES>;
+    if constexpr (Registers<DAP>::kShares) {
+        static std::atomic<bool> fits{false};
+        const cudaError_t r = check_registers(kernel, kThreads, Registers<DAP>::kShare, fits);
+        if (r != cudaSuccess) return r;
+    }
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(l.c.batch * l.c.heads * slabs), STATES ? l.c.segments - 1 : l.c.segments, l.runs);

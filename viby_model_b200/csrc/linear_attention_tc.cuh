@@ -56,6 +56,8 @@ using tma::smem_u32;
 constexpr int kC = 128;               // tokens of a chunk
 constexpr int kThreads = 768;
 constexpr int kSmallRegs = 64, kLargeRegs = 112;  // four groups and two: six times the 80 of the launch
+constexpr int kRegisterShare = 4 * 128 * kSmallRegs + 2 * 128 * kLargeRegs;
+static_assert(kRegisterShare <= 65536, "registers of an SM");
 constexpr int kWeighers = 256;
 constexpr int kWholeChunks = 4096;  // chunks that are looked over beforehand; later ones count as not whole
 constexpr int kPow = kC + 2;          // a^0 .. a^(kC + 1)
@@ -848,7 +850,10 @@ cudaError_t launch(const Launch& given, unsigned int* timeouts, cudaStream_t s) 
             return cudaErrorNotSupported;
     }
     auto kernel = k_linear_tc<ROWS, STATES, REV>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<bool> fits{false};
+    cudaError_t e = check_registers(kernel, kThreads, kRegisterShare, fits);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(l.c.batch * l.c.heads * slabs), STATES ? l.c.segments - 1 : l.c.segments, l.runs);
     note_launch(STATES ? "linear_tc_states" : "linear_tc");

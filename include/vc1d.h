@@ -376,7 +376,8 @@ typedef struct vc1d_linear_args {
     void* workspace;
     int64_t workspace_bytes;
     int32_t segments;       /* parts of the time axis: 0 = automatic */
-    int32_t reserved;
+    int32_t test_expire;    /* self-test of the bounded waits: n > 0 = the tcgen05 kernel withholds the n-th chunk of every
+                             * part, so that waits run out (vc1d_tma_timeouts) and results are incomplete.  Otherwise 0 */
 } vc1d_linear_args;
 
 VC1D_API int vc1d_linear(const vc1d_linear_args* args, void* stream);

@@ -77,3 +77,64 @@ def test_calls_without_tokens_copy_the_state(dtype, D, kernel):
         assert V.last_kernel() == "linear_simt"
         assert all(x.shape == y.shape for x, y in zip(grads, (q, k, v)))
         assert torch.equal(di, ds if dfinal is not None else torch.zeros_like(ds))
+
+
+def test_waits_of_the_tcgen05_kernel_run_out_and_report():
+    """With the self-test's chunk withheld, the warps that wait for it give up, the others follow, the CTA waits for its
+    products and copies in flight and frees its tensor memory: the launch returns, the count of expired waits grows, and
+    the next ordinary launch is clean.  For one and two buffers of keys (heads of 160 and 64), both directions, the pass that
+    finds the parts' states, rows with and without masks, and the first, second and a later chunk.  In a process of its
+    own: the count stays."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    code = r"""
+import ctypes as C
+import torch
+import viby_model_b200 as V
+from viby_model_b200 import _cabi, linear_attention as la
+for D, masked, runs in ((64, 0, ((1, 1), (1, 4))), (64, 1, ((2, 3),)), (160, 1, ((1, 2), (1, 4))), (160, 0, ((2, 2),))):
+    g = torch.Generator().manual_seed(D)
+    T, H = 900, 2
+    q, k, v, do = (torch.randn(2, T, H, D, generator=g).bfloat16().cuda() for _ in range(4))
+    ld = torch.tensor([-0.01, -0.3]).cuda()
+    m = (torch.rand(2, T, generator=g) < 0.8).cuda() if masked else None
+    for segments, chunk in runs:
+        want = V.linear_attention_fn(q, k, v, ld, None, None, True, attention_mask=m, kernel="tc", segments=segments)
+        grads = V.linear_attention_bwd(q, k, v, ld, do, attention_mask=m, kernel="tc", segments=segments)
+        assert V.last_kernel() == "linear_tc"
+        stream = torch.cuda.current_stream().cuda_stream
+        before = V.tma_timeouts()
+        a, keep = la._fill(q, k, v, ld, None, None, m, None, "tc", segments)
+        out, state = torch.zeros_like(want[0]), torch.zeros_like(want[1])
+        a.out, a.out_strides[:], a.final_state, a.final_strides[:] = out.data_ptr(), out.stride(), state.data_ptr(), state.stride()
+        a.test_expire = chunk
+        ws = la._workspace(a, _cabi.lib.vc1d_linear_workspace, q.device)
+        assert _cabi.lib.vc1d_linear(C.byref(a), stream) == 0
+        torch.cuda.synchronize()  # the launch returns: nothing hangs, nothing traps
+        between = V.tma_timeouts()
+        assert between > before, "the expired waits were not reported"
+        b = _cabi.LinearBwdArgs()
+        b.struct_size, b.segments, b.f, b.dout = C.sizeof(b), segments, a, do.data_ptr()
+        b.dout_strides[:] = do.stride()
+        new = [torch.zeros_like(x) for x in (q, k, v)]
+        b.dq, b.dk, b.dv = (x.data_ptr() for x in new)
+        b.dq_strides[:], b.dk_strides[:], b.dv_strides[:] = (x.stride() for x in new)
+        ws2 = la._workspace(b, _cabi.lib.vc1d_linear_bwd_workspace, q.device)
+        assert _cabi.lib.vc1d_linear_bwd(C.byref(b), stream) == 0
+        torch.cuda.synchronize()
+        expired = V.tma_timeouts()
+        assert expired > between
+        o, s = V.linear_attention_fn(q, k, v, ld, None, None, True, attention_mask=m, kernel="tc", segments=segments)
+        again = V.linear_attention_bwd(q, k, v, ld, do, attention_mask=m, kernel="tc", segments=segments)
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[0]) and torch.equal(s, want[1])
+        assert all(torch.equal(x, y) for x, y in zip(again[:3], grads[:3]))
+        assert V.tma_timeouts() == expired, "an ordinary launch after the self-test reported expired waits"
+print("EXPIRED", expired)
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=str(ROOT))
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "EXPIRED" in r.stdout

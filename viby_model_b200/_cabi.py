@@ -257,7 +257,7 @@ class LinearArgs(C.Structure):
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_int64),
         ("segments", C.c_int32),
-        ("reserved", C.c_int32),
+        ("test_expire", C.c_int32),
     ]
 
 

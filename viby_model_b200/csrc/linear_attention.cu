@@ -167,6 +167,7 @@ Common common_of(const vc1d_linear_args& a) {
     c.batch = a.batch;
     c.heads = a.heads;
     c.seqlen = a.seqlen;
+    c.test_expire = a.test_expire;
     return c;
 }
 

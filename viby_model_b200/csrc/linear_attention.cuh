@@ -60,6 +60,7 @@ struct Common {
     int batch, heads, seqlen;
     int segments;               // time is split into this many parts of seg_chunks chunks
     int seg_chunks;
+    int test_expire;            // self-test: the chunk, counted from 1, that kTc withholds; 0 = none
     // workspace of a split launch, per run: [segments - 1][batch * heads][da * dv] states, then factors (hi, lo)
     float* seg_state[3];
     float2* seg_factor[3];

@@ -63,7 +63,10 @@ constexpr int kWholeChunks = 4096;  // chunks that are looked over beforehand; l
 constexpr int kPow = kC + 2;          // a^0 .. a^(kC + 1)
 constexpr int kCols = 64;             // columns of a slab
 constexpr int kPanel = kC * 128;      // bytes of a panel of 128 rows
-constexpr unsigned kSpin = 1u << 22;  // polls of 64 ns and more
+
+// Polls after which a wait gives up: about a second, where a chunk takes microseconds.  A poll that fails takes 1.6 us and more:
+// try_wait itself waits (1.5 us measured), and a sleep of 64 ns follows.  A constant: as an argument it costs spills.
+constexpr unsigned kMaxPolls = 1u << 18;
 
 // TMEM columns
 // P has two buffers, for even and odd chunks, so that the next chunk's products need not wait for this one's decays.  The
@@ -196,7 +199,7 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 // A bounded wait.
 __device__ __forceinline__ bool poll(uint32_t addr, uint32_t parity, volatile uint32_t* dead, unsigned int* timeouts) {
 #pragma unroll 1
-    for (unsigned i = 0; i < kSpin; ++i) {
+    for (unsigned i = 0; i < kMaxPolls; ++i) {
         if (mbar_test(addr, parity)) return true;
         if (*dead) return false;
         if (i > 64) __nanosleep(64);
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     float* pw_lo = pw_hi + kPow;
     float* add = reinterpret_cast<float*>(sm + L::kAdd);
     Info* infos = reinterpret_cast<Info*>(sm + L::kInfo);
-    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4-6] chunks asked for
+    uint32_t* misc = reinterpret_cast<uint32_t*>(sm + L::kMisc);  // [0] TMEM address, [1] a wait expired, [2-3] a last barrier, [4-6] chunks asked for, [7] chunks announced
     volatile uint32_t* dead = misc + 1;
 
     const Run& r = l.run[blockIdx.z];
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         for (int i = tid; i < NS * kPanel / 16; i += kThreads)
             *reinterpret_cast<uint4*>(sm + L::kK + (i / (kPanel / 16) * L::kPanels + p) * kPanel + i % (kPanel / 16) * 16) = make_uint4(0, 0, 0, 0);
     if (tid == 0) {
-        misc[1] = misc[4] = misc[5] = misc[6] = 0;
+        misc[1] = misc[4] = misc[5] = misc[6] = misc[7] = 0;
         for (int i = 0; i < 2; ++i) {
             for (int x = 0; x < 3; ++x) {
                 mbar_init(bar(kTmaQ + x, i), 1);
@@ -727,6 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
         }
 #pragma unroll 1
         for (int ch = 0; warp == 23 && ch < chunks; ++ch) {
+            if (ch + 1 == c.test_expire) break;  // the self-test's missing chunk
             // nobody looks at the chunk before the last but one any more
             if (ch >= 2 && !(wait_warp(kKvFree, ch - 2) && (STATES || wait_warp(kPvDone, ch - 2)))) break;
             const int t0 = first_token(ch);
@@ -761,6 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
                 if (!STATES) mbar_arrive(bar(kPRaw, ch));
                 mbar_arrive(bar(kKvDone, ch));
                 mbar_arrive(bar(kVFull, ch));
+                misc[7] = ch + 1;
             }
             if (!to_clear(ch)) continue;
             bool ok = true;
@@ -789,18 +794,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     __syncthreads();
     if (warp == 20) {
         fence_after();
-        if (*dead && lane == 0) {
+        const bool issuer = elect_lane();  // a commit speaks for the products of its own thread only
+        if (*dead && issuer) {
             // products and copies may still be under way: they end by themselves, and TMEM and shared memory have to
-            // outlive them.  A barrier of its own for the products; the copies' barriers for the copies.
+            // outlive them.  A barrier of its own for the products; the copies' barriers for the copies.  That of the values
+            // also wants the chunk's announcement, which may never have come.
             const uint32_t last = base + L::kMisc + 8;
             mbar_init(last, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             commit(true, last);
-            for (unsigned i = 0; i < kSpin && !mbar_test(last, 0); ++i) __nanosleep(64);
+            for (unsigned i = 0; i < kMaxPolls && !mbar_test(last, 0); ++i) __nanosleep(64);
             for (int what = 0; what < 3; ++what) {
                 const int asked = misc[4 + what];
-                for (int ch = max(0, asked - 2); ch < asked; ++ch)
-                    for (unsigned i = 0; i < kSpin && !mbar_test(bar((to_clear(ch) ? kTmaQ : kQFull) + what, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+                for (int ch = max(0, asked - 2); ch < asked; ++ch) {
+                    if (what == 2 && ch >= (int)misc[7] && !to_clear(ch)) mbar_arrive(bar(kVFull, ch));
+                    for (unsigned i = 0; i < kMaxPolls && !mbar_test(bar((to_clear(ch) ? kTmaQ : kQFull) + what, ch), (uint32_t)(ch >> 1) & 1u); ++i) __nanosleep(64);
+                }
             }
         }
         __syncwarp();

@@ -138,3 +138,26 @@ print("EXPIRED", expired)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=str(ROOT))
     assert r.returncode == 0, r.stdout + r.stderr
     assert "EXPIRED" in r.stdout
+
+
+def test_new_forms_are_remembered_after_hundreds_of_others(monkeypatch):
+    """Prompts of 300 lengths and batches of 300 sizes, as a server sees them: the form that comes next is prepared once, and the
+    number of those that are kept is bounded."""
+    from viby_model_b200 import linear_attention as la
+
+    q, k, v, _, s0, _ = (x.to(DEV) for x in make(1, 402, 1, 1, 1, 8, 8, torch.bfloat16))
+    g = decays(1).to(DEV)
+    state = s0.expand(402, -1, -1, -1).contiguous()
+    for n in range(1, 301):
+        V.linear_attention_fn(q[:, :n], k[:, :n], v[:, :n], g)
+        V.linear_attention_update(q[0, :n], k[0, :n], v[0, :n], state[:n], g)
+    checked = []
+    for name in ("_check_heads", "_fill"):
+        monkeypatch.setattr(la, name, lambda *a, f=getattr(la, name), name=name: (checked.append(name), f(*a))[1])
+    for n in (401, 402):
+        for turn in range(3):
+            V.linear_attention_fn(q[:, :n], k[:, :n], v[:, :n], g)
+            V.linear_attention_update(q[0, :n], k[0, :n], v[0, :n], state[:n], g)
+            assert checked == (["_fill", "_check_heads", "_check_heads"] if turn == 0 else []), (n, turn)
+            checked.clear()
+    assert len(la._prepared("linear_args")) <= 256 and len(la._prepared("linear_update_args")) <= 256

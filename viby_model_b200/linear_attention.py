@@ -87,6 +87,17 @@ def _prepared(kind: str) -> dict:
     return cache
 
 
+_MAX_FORMS = 256  # of a kind and thread
+
+
+def _remember(forms: dict, key, value) -> None:
+    """Keeps a prepared struct; the oldest makes room, because prompt lengths that do not come back would else fill the place
+    for good."""
+    if len(forms) >= _MAX_FORMS:
+        del forms[next(iter(forms))]
+    forms[key] = value
+
+
 def _same_device(t: torch.Tensor, device, what: str) -> None:
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, q on {device}")
@@ -200,8 +211,8 @@ def _forward(q, k, v, log_decay, seq_idx, initial_states, return_final_states, f
     _cabi.check(st, "linear_attention_fn")
     _changed(out, state)
     # workspace sizes and kernels depend on the alignment of the data too: only aligned calls are remembered, for aligned calls
-    if key is not None and len(_prepared("linear_args")) < 256 and _aligned(q, k, v):
-        _prepared("linear_args")[key] = (a, 0 if ws is None else ws.numel())
+    if key is not None and _aligned(q, k, v):
+        _remember(_prepared("linear_args"), key, (a, 0 if ws is None else ws.numel()))
     del keep, ws
     return out, state
 
@@ -469,6 +480,6 @@ def _update(q, k, v, state, log_decay, attention_mask, scale, out):
     st = _launch(q.device, _cabi.lib.vc1d_linear_update, C.byref(a), _stream_handle(q.device))
     _cabi.check(st, "linear_attention_update")
     _changed(state, out)
-    if key is not None and len(_prepared("linear_update_args")) < 256:
-        _prepared("linear_update_args")[key] = a
+    if key is not None:
+        _remember(_prepared("linear_update_args"), key, a)
     return out

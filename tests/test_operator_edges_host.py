@@ -158,3 +158,16 @@ def test_states_whose_requests_share_memory_are_refused(strides, ok):
     before = _cabi.launch_count()
     assert _cabi.lib.vc1d_linear_update(C.byref(a), None) == (_cabi.VC1D_E_ALIAS if ok else _cabi.VC1D_E_STRIDE)
     assert _cabi.launch_count() == before
+
+
+@pytest.mark.parametrize("shape", [((1 << 32) + 8, 1, 1), (1, (1 << 32) + 8, 1), (1, 1, (1 << 32) + 2), ((1 << 31), 1, 1)])
+def test_axes_that_do_not_fit_the_call_are_refused(shape):
+    """They would be cut to 32 bits: 2^32 + 8 rows became 8, and the other outputs stayed unwritten."""
+    x = torch.zeros(1, 1, 1, 1).expand(*shape, 1)
+    with pytest.raises(ValueError, match="too large"):
+        V.linear_attention_fn(x, x, x, torch.zeros(1).expand(shape[2]))
+    with pytest.raises(ValueError, match="too large"):
+        V.linear_attention_bwd(x, x, x, torch.zeros(1).expand(shape[2]), x)
+    t = x.squeeze(1) if shape[1] == 1 else x.squeeze(0)
+    with pytest.raises(ValueError, match="too large"):
+        V.linear_attention_update(t, t, t, t.unsqueeze(-1), torch.zeros(1).expand(t.shape[1]))

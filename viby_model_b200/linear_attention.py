@@ -38,6 +38,8 @@ def _check_heads(q, k, v, lead: int, what: str):
             raise ValueError(f"{name} shape {tuple(x.shape)} does not match q shape {tuple(q.shape)} in {what}")
     H, Dk = q.shape[lead:]
     Hk, Hv, Dv = k.shape[lead], v.shape[lead], v.shape[lead + 1]
+    if max(H, *q.shape[:lead]) > 0x7fffffff:  # more than the fields of the C structs hold
+        raise ValueError(f"q shape {tuple(q.shape)} is too large: at most 2^31 - 1 along an axis")
     if k.shape[lead + 1] != Dk:
         raise ValueError(f"k dim {k.shape[lead + 1]} does not match q dim {Dk}")
     if H < 1 or Hk < 1 or Hv < 1 or H % Hk != 0 or H % Hv != 0:

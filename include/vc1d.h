@@ -447,6 +447,7 @@ VC1D_API uint32_t vc1d_sizeof_linear_update_args(void);
  */
 #define VC1D_PAGES_MAX_TENSORS 128
 #define VC1D_PAGES_MAX_PAGES 8192
+#define VC1D_PAGES_MAX_ENTRIES (1 << 30)
 enum { VC1D_PAGES_REORDER = 0, VC1D_PAGES_COPY = 1, VC1D_PAGES_FREE = 2, VC1D_PAGES_COMPACT = 3 };
 
 typedef struct vc1d_page_tensor {
@@ -466,7 +467,7 @@ typedef struct vc1d_pages_args {
     const uint8_t* live;    /* device: COMPACT live[pages] */
     int32_t* new_index;     /* device: COMPACT, [pages] */
     int32_t* count;         /* device: COMPACT, [1] */
-    int32_t n;              /* COPY, FREE: entries */
+    int32_t n;              /* COPY, FREE: entries, 0..VC1D_PAGES_MAX_ENTRIES */
     int32_t index_dtype;    /* of source and dst: VC1D_I32 | VC1D_I64 */
 } vc1d_pages_args;
 

@@ -171,3 +171,18 @@ def test_axes_that_do_not_fit_the_call_are_refused(shape):
     t = x.squeeze(1) if shape[1] == 1 else x.squeeze(0)
     with pytest.raises(ValueError, match="too large"):
         V.linear_attention_update(t, t, t, t.unsqueeze(-1), torch.zeros(1).expand(t.shape[1]))
+
+
+def test_lists_of_too_many_pages_are_refused():
+    """At most 2^30 entries: the kernel's and the call's counters are 32 bits wide."""
+    long = torch.zeros(1, dtype=torch.int32).expand((1 << 32) + 5)
+    for call in (lambda: V.free_pages([], long), lambda: V.copy_pages([], long, long), lambda: V.reorder_pages([], long),
+                 lambda: V.free_pages([], long[: (1 << 30) + 1])):
+        with pytest.raises(ValueError, match="at most"):
+            call()
+    before = _cabi.launch_count()
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        for op in (_cabi.PAGES_COPY, _cabi.PAGES_FREE):
+            a = page_args([(FAKE, 64, 64)], op=op, n=n, dst=16 * FAKE, source=1 << 40)
+            assert _cabi.lib.vc1d_pages(C.byref(a), None) == _cabi.VC1D_E_TOO_LARGE
+    assert _cabi.launch_count() == before

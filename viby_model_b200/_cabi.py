@@ -25,7 +25,8 @@ VC1D_E_STRIDE, VC1D_E_STRUCT, VC1D_E_ACTIVATION, VC1D_E_ALIAS, VC1D_E_TOO_LARGE 
 KERNEL_AUTO, KERNEL_CHANNEL_LAST, KERNEL_TIME_MAJOR, KERNEL_GENERIC, KERNEL_TMA = 0, 1, 2, 3, 4
 LINEAR_KERNEL_BY_NAME = {None: 0, "auto": 0, "simt": 1, "mma": 2, "tc": 3}
 LINEAR_MAX_DIM = 256  # VC1D_LINEAR_MAX_DIM
-PAGES_MAX_TENSORS, PAGES_MAX_PAGES = 128, 8192  # VC1D_PAGES_MAX_TENSORS, VC1D_PAGES_MAX_PAGES
+# VC1D_PAGES_MAX_TENSORS, VC1D_PAGES_MAX_PAGES, VC1D_PAGES_MAX_ENTRIES
+PAGES_MAX_TENSORS, PAGES_MAX_PAGES, PAGES_MAX_ENTRIES = 128, 8192, 1 << 30
 PAGES_REORDER, PAGES_COPY, PAGES_FREE, PAGES_COMPACT = 0, 1, 2, 3
 KERNEL_BY_NAME = {
     None: KERNEL_AUTO,

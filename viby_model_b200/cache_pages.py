@@ -129,6 +129,8 @@ class PageTable:
             raise ValueError(f"{what} must be a 1D tensor")
         if t.dtype not in _INDEX_DTYPES:
             raise ValueError(f"{what} must be int32 or int64, got {t.dtype}")
+        if t.shape[0] > _cabi.PAGES_MAX_ENTRIES:
+            raise ValueError(f"{what} has {t.shape[0]} entries, at most {_cabi.PAGES_MAX_ENTRIES}")
         if self.device is not None and t.device != self.device:
             raise ValueError(f"{what} is on {t.device}, the states on {self.device}")
         return t.contiguous()

@@ -23,6 +23,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTensors = VC1D_PAGES_MAX_TENSORS;
 constexpr int kMaxPages = VC1D_PAGES_MAX_PAGES;
+constexpr int kMaxEntries = VC1D_PAGES_MAX_ENTRIES;  // a thread's step past the last one stays within 32 bits
 
 // Dynamic shared memory of a launch: the list of moves, and a staging area.  48 KB keep four CTAs on an SM; many pages take
 // more, so that a strip is at least a 16-byte column of all of them.
@@ -255,7 +256,7 @@ VC1D_API int vc1d_pages(const vc1d_pages_args* a, void* stream) {
     if (a->struct_size != sizeof(vc1d_pages_args)) return VC1D_E_STRUCT;
     if (a->op < VC1D_PAGES_REORDER || a->op > VC1D_PAGES_COMPACT) return VC1D_E_SHAPE;
     if (a->pages < 0 || a->n_tensors < 0 || a->n < 0) return VC1D_E_SHAPE;
-    if (a->pages > kMaxPages || a->n_tensors > kMaxTensors) return VC1D_E_TOO_LARGE;
+    if (a->pages > kMaxPages || a->n_tensors > kMaxTensors || a->n > kMaxEntries) return VC1D_E_TOO_LARGE;
     const bool compact = a->op == VC1D_PAGES_COMPACT, listed = a->op == VC1D_PAGES_COPY || a->op == VC1D_PAGES_FREE;
     if (!compact && a->index_dtype != VC1D_I32 && a->index_dtype != VC1D_I64) return VC1D_E_DTYPE;
     if (compact && (a->count == nullptr || (a->pages > 0 && (a->live == nullptr || a->new_index == nullptr)))) return VC1D_E_NULL;

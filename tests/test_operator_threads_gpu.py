@@ -56,3 +56,43 @@ def test_linear_attention_of_small_and_of_large_heads(segments):
     want = [c() for c in calls]
     for o, w in zip(in_two_threads(calls, 1500), want):
         assert torch.equal(o, w)
+
+
+def first_call_of_a_thread(call):
+    got = []
+
+    def work():
+        try:
+            got.append(call())
+        except Exception as e:  # noqa: BLE001  (reported by the test)
+            got.append(e)
+
+    torch.cuda.synchronize()
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    if isinstance(got[0], Exception):
+        raise got[0]
+    return got[0]
+
+
+@pytest.mark.parametrize("kernel", ["tc", "mma", "simt"])
+def test_the_first_cuda_call_of_a_host_thread(kernel):
+    """No context is bound to a new thread yet, and memory comes from the allocator's cache: the call has to bind it."""
+    q, k, v, do, s0, ds = (x.to(DEV) for x in make(1, 300, 2, 2, 2, 64, 64, torch.bfloat16))
+    g = decays(2).to(DEV)
+    calls = [lambda: V.linear_attention_fn(q, k, v, g, None, s0, True, kernel=kernel),
+             lambda: V.linear_attention_bwd(q, k, v, g, do, None, s0, ds, kernel=kernel),
+             lambda: (V.linear_attention_update(q[:, 0], k[:, 0], v[:, 0], s0.clone(), g),)]
+    for call in calls:
+        want = call()
+        for a, b in zip(first_call_of_a_thread(call), want):
+            assert torch.equal(a, b)
+
+
+def test_the_first_convolution_of_a_host_thread():
+    x, w = torch.randn(4, 512, 1152, device=DEV).bfloat16().transpose(1, 2), torch.randn(1152, 4, device=DEV).bfloat16()
+    for call in (lambda: (V.causal_conv1d_fn(x, w, None, activation="silu", kernel="tma"),), lambda: V.causal_conv1d_bwd(x, w, None, x, "silu")[:1]):
+        want = call()
+        for a, b in zip(first_call_of_a_thread(call), want):
+            assert torch.equal(a, b)

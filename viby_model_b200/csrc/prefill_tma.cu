@@ -11,7 +11,9 @@ namespace tma {
 __device__ unsigned int g_tma_timeouts = 0;
 
 EncodeFn encode_fn() {
+    using CurrentFn = CUresult (*)(CUcontext*);
     static EncodeFn fn = nullptr;
+    static CurrentFn current = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
         void* sym = nullptr;
@@ -19,7 +21,14 @@ EncodeFn encode_fn() {
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeFn>(sym);
+        if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &sym, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            current = reinterpret_cast<CurrentFn>(sym);
     });
+    // The encoder is a driver call and wants a current context.  A host thread (autograd's, a server's) gets the device's with
+    // its first runtime call that needs it, which may be the launch that the tensor maps are for.
+    CUcontext ctx = nullptr;
+    int dev = 0;
+    if (current != nullptr && current(&ctx) == CUDA_SUCCESS && ctx == nullptr && cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
     return fn;
 }
 

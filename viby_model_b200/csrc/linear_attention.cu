@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(256) k_linear_join(const __grid_constant__ Lau
             for (int j = 0; j < 8; ++j) {
                 if (s0 + j < parts) {
                     // factor 0 is a sequence that ended inside the part: whatever came before is gone, infinities too
-                    x = f[j].x == 0.f ? z[j] : fmaf(x, f[j].x, fmaf(x, f[j].y, z[j]));
+                    // a second half of 0 (a part without a token: the factor 1) adds nothing, where infinity * 0 would
+                    x = f[j].x == 0.f ? z[j] : fmaf(x, f[j].x, f[j].y == 0.f ? z[j] : fmaf(x, f[j].y, z[j]));
                     state[(s0 + j) * all + i] = x;
                 }
             }

@@ -541,7 +541,8 @@ __global__ void __launch_bounds__(kThreads, DAP == 256 ? 1 : 2) k_linear_mma(con
         if (chunk + 1 < chunks) load_kv(chunk + 1);
         cp_commit();
         const bool more = chunk + 1 < chunks;
-        if (more || want_last) {
+        // without a token the state stays, whatever it holds: not even times 1 + 0
+        if ((more || want_last) && infos[chunk % 3].n_all != 0) {
             const Info& f = infos[chunk % 3];
             const T* sk = sm + L::kK + (chunk & 1) * kChunk * L::kStrideA;
             const T* sv = sm + L::kV + (chunk & 1) * kChunk * L::kStrideV;

@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_simt(const __grid_consta
         // the state: X' = a^{n_C} X + sum_j w_j k_j v_j^T
         __syncthreads();  // the queries have read it
         const float2 f = pw[n_all];
-        for (int i0 = tid / 16 * 4; i0 < dap; i0 += kThreads / 16 * 4) {
+        // without a token the state stays, whatever it holds: not even times 1 + 0
+        for (int i0 = n_all == 0 ? dap : tid / 16 * 4; i0 < dap; i0 += kThreads / 16 * 4) {
             float acc[4][4] = {};
 #pragma unroll 4
             for (int j = 0; j < kChunk; ++j) {

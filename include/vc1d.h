@@ -336,6 +336,8 @@ VC1D_API uint32_t vc1d_sizeof_update_bwd_args(void);
  *     valid token:   S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t
  *     masked token:  S_t = S_{t-1},                 o_t = 0      (its q, k, v are not read)
  *     packed rows:   S starts at zero at the first token of each run of equal seq_idx
+ * An infinity or NaN of a valid token may reach earlier tokens of its row in the same chunk (64 or 128 tokens) as NaN; in
+ * packed rows it stays in its sequence, behind the token that has it.
  * States are fp32 [batch, heads, dim_k, dim_v].  heads is a multiple of heads_k and of heads_v; head h reads key head
  * h / (heads / heads_k) and value head h / (heads / heads_v).  Head dimensions 1..VC1D_LINEAR_MAX_DIM.
  * Sums, powers of the decay and states are fp32; out is rounded once.  In the 16-bit tensor-core kernel the products

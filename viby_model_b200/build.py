@@ -42,6 +42,7 @@ SOURCES = [
     "linear_attention_mma_f16.cu",
     "linear_attention_tc.cu",
     "linear_attention_update.cu",
+    "linear_attention_isolate.cu",
     "cache_pages.cu",
 ]
 

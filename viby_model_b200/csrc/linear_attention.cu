@@ -276,7 +276,10 @@ cudaError_t enqueue(Launch& l, int dtype, int kernel, int segments, char* ws, lo
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }
-    return launch_one(l, dtype, kind, false, s);
+    const bool packed = l.c.seq_idx != nullptr && l.c.seqlen > 0;
+    if (packed) note_launch("linear_isolate");  // counted here: the name that stays is the main kernel's
+    cudaError_t e = launch_one(l, dtype, kind, false, s);
+    return e == cudaSuccess && packed ? launch_linear_isolate(l, dtype, s) : e;
 }
 
 Launch forward_launch(const vc1d_linear_args& a) {

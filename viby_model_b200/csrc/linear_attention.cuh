@@ -236,5 +236,7 @@ cudaError_t launch_linear_mma_bf16(const lin::Launch& l, bool states_only, cudaS
 cudaError_t launch_linear_mma_f16(const lin::Launch& l, bool states_only, cudaStream_t s);
 // bf16, as above and at most 160 state rows in every run.
 cudaError_t launch_linear_tc(const lin::Launch& l, bool states_only, cudaStream_t s);
+// Packed rows, after the outputs: replaces what bad values of one sequence left in the others.
+cudaError_t launch_linear_isolate(const lin::Launch& l, int dtype, cudaStream_t s);
 
 }  // namespace vc1d

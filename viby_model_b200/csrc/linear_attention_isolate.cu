@@ -1,0 +1,200 @@
+// Packed rows: keeps the infinities and NaN of one sequence out of the others.
+//
+// The kernels take a chunk's products at once: a pair of tokens of different sequences, or of a query and a later key, has the
+// weight 0, and 0 times a value that is not finite is NaN.  So a bad value of one request would reach its neighbours in the
+// chunk, and through the state all of the request that follows.  What it leaves there is always NaN, never infinity, and it is
+// rare: this kernel looks the outputs over and, where a token has a NaN although no key or value of its own sequence up to
+// it is to blame, runs the recurrence for it as it is written,
+//     Y_t = a Y_{t-1} + s k_t v_t^T,   o_t = q_t^T Y_t     from the sequence's first token,
+// and replaces the NaN.  All other outputs stay as they are.
+//
+// Bound by its launch and by reading the outputs.  A CTA takes 256 tokens of one (row, head, slab of 64 columns).  24567 tokens
+// of 8 heads of 64 in fp16, 25 MB: 10 us behind a main kernel of 102; 300 tokens: 3 us.  Registers for two CTAs an SM: with
+// four or six the clean case takes the same time, and the recurrence, which costs about a microsecond a token and runs
+// only behind a neighbour's bad value, spills.
+#include "linear_attention.cuh"
+
+namespace vc1d {
+namespace lin {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPart = kThreads;  // tokens of a CTA
+constexpr int kSlab = 64;
+constexpr int kRowsEach = kMaxDim / (kThreads / kSlab);  // state rows of a thread
+
+__device__ __forceinline__ bool is_nan(float x) { return x != x; }
+__device__ __forceinline__ bool is_nan(__nv_bfloat16 x) { return (__bfloat16_as_ushort(x) & 0x7fffu) > 0x7f80u; }
+__device__ __forceinline__ bool is_nan(__half x) { return (__half_as_ushort(x) & 0x7fffu) > 0x7c00u; }
+
+// This thread's share of the rows first .. last - 1 (at most kPart): 16 bytes of every so many rows, all a few of them asked for at once.
+template <typename O>
+__device__ __forceinline__ bool nan_in_rows(const O* o, long long stride, int first, int last, int cols) {
+    constexpr int kPer = 16 / (int)sizeof(O), kAcross = kSlab / kPer, kDown = kThreads / kAcross, kSteps = kPart / kDown, kBatch = 8;
+    const int at = (int)threadIdx.x % kAcross * kPer, row = first + (int)threadIdx.x / kAcross;
+    if (at >= cols) return false;
+    bool bad = false;
+#pragma unroll
+    for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+        uint4 x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int t = row + (s0 + i) * kDown;
+            x[i] = t < last ? *reinterpret_cast<const uint4*>(o + (long long)t * stride + at) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const O* y = reinterpret_cast<const O*>(&x[i]);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) bad |= is_nan(y[j]);
+        }
+    }
+    return bad;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 2) k_linear_isolate(const __grid_constant__ Launch l, int pieces, int slabs_most) {
+    using E = Elem<DT>;
+    using T = typename E::type;
+    __shared__ float key[kMaxDim], query[kMaxDim], sums[kThreads / kSlab][kSlab];
+    __shared__ int found;
+    griddep_wait();
+    const Run& r = l.run[blockIdx.z];
+    const Common& c = l.c;
+    const int tid = threadIdx.x, slabs = (r.dv + kSlab - 1) / kSlab;
+
+    for (int piece = blockIdx.y; piece < pieces; piece += gridDim.y) {  // row, head and slab
+        const int slab = piece % slabs_most, bh = piece / slabs_most;
+        if (slab >= slabs) continue;  // a run with fewer slabs than the launch's widest
+        const int b = bh / c.heads, h = bh % c.heads, c0 = slab * kSlab, cols = min(kSlab, r.dv - c0);
+        const int i0 = blockIdx.x * kPart, i1 = min(c.seqlen, i0 + kPart);  // tokens in the run's order
+        const T* pa = static_cast<const T*>(r.a.p) + (long long)b * r.a.sb + (long long)(h / r.a.group) * r.a.sh;
+        const T* pk = static_cast<const T*>(r.k.p) + (long long)b * r.k.sb + (long long)(h / r.k.group) * r.k.sh;
+        const T* pv = static_cast<const T*>(r.v.p) + (long long)b * r.v.sb + (long long)(h / r.v.group) * r.v.sh + (long long)c0 * r.v.sd;
+        const long long out0 = (long long)b * r.o.sb + (long long)h * r.o.sh + (long long)c0 * r.o.sd;
+        float* o32 = static_cast<float*>(const_cast<void*>(r.o.p));
+        T* o16 = static_cast<T*>(const_cast<void*>(r.o.p));
+        auto out_is_nan = [&](int i, int col) {
+            const long long at = out0 + (long long)i * r.o.st + (long long)col * r.o.sd;
+            const float x = r.out_f32 ? o32[at] : E::to_float(o16[at]);
+            return x != x;
+        };
+        // whether any output of the tokens first .. last - 1 is NaN; one answer for the CTA
+        auto nan_among = [&](int first, int last) {
+            bool bad = false;
+            if (r.out_vec && r.dv % 8 == 0) {
+                bad = r.out_f32 ? nan_in_rows<float>(o32 + out0, r.o.st, first, last, cols) : nan_in_rows<T>(o16 + out0, r.o.st, first, last, cols);
+            } else {
+                for (int e = tid; e < (last - first) * cols; e += kThreads) bad |= out_is_nan(first + e / cols, e % cols);
+            }
+            return __syncthreads_or(bad) != 0;
+        };
+        if (!nan_among(i0, i1)) continue;
+
+        auto starts = [&](int i) {  // whether a sequence starts at token i
+            if (i == 0) return true;
+            const long long at = r.reverse ? c.seqlen - 1 - i : i;
+            const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + at * c.seq_st;
+            return p[0] != (r.reverse ? p[c.seq_st] : p[-c.seq_st]);
+        };
+        for (int p0 = i0, p1; p0 < i1; p0 = p1) {  // the sequences of the part
+            __syncthreads();
+            if (tid == 0) found = i1;
+            __syncthreads();
+            const int next = p0 + 1 + tid;
+            if (next < i1 && starts(next)) atomicMin(&found, next);
+            __syncthreads();
+            p1 = found;
+            if (!nan_among(p0, p1)) continue;
+            int first = p0;  // of the sequence
+            for (int hi = p0; p0 == i0; hi -= kThreads) {
+                __syncthreads();
+                if (tid == 0) found = -1;
+                __syncthreads();
+                if (hi - tid >= 0 && starts(hi - tid)) atomicMax(&found, hi - tid);
+                __syncthreads();
+                first = found;
+                if (first >= 0) break;
+            }
+            // the sequence's first token with a key, or a value of this slab, that is not finite
+            int end = p1;
+            for (int t0 = first; t0 < p1 && end == p1; t0 += kThreads / 32) {
+                const int t = t0 + (tid >> 5);
+                bool bad = false;
+                if (t < p1) {
+                    for (int d = tid & 31; d < r.da; d += 32) bad = bad || !isfinite(E::to_float(pk[(long long)t * r.k.st + d * r.k.sd]));
+                    for (int d = tid & 31; d < cols; d += 32) bad = bad || !isfinite(E::to_float(pv[(long long)t * r.v.st + d * r.v.sd]));
+                }
+                __syncthreads();
+                if (tid == 0) found = p1;
+                __syncthreads();
+                if (bad) atomicMin(&found, t);
+                __syncthreads();
+                end = found;
+            }
+            if (end <= p0 || !nan_among(p0, end)) continue;
+
+            const int col = tid % kSlab, group = tid / kSlab;
+            const double e = exp((double)c.log_decay[h]);
+            const float hi = (float)e, lo = isfinite(hi) ? (float)(e - (double)hi) : 0.f;
+            float Y[kRowsEach] = {};
+            for (int t = first; t < end; ++t) {
+                __syncthreads();  // key, query and sums have been read
+                if (tid < kMaxDim) {
+                    key[tid] = tid < r.da ? E::to_float(pk[(long long)t * r.k.st + tid * r.k.sd]) : 0.f;
+                    query[tid] = tid < r.da && t >= p0 ? E::to_float(pa[(long long)t * r.a.st + tid * r.a.sd]) : 0.f;
+                }
+                __syncthreads();
+                const float v = col < cols ? E::to_float(pv[(long long)t * r.v.st + col * r.v.sd]) * r.s_pair : 0.f;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < kRowsEach; ++i) {
+                    if (group * kRowsEach + i < r.da) {
+                        Y[i] = fmaf(Y[i], hi, fmaf(Y[i], lo, key[group * kRowsEach + i] * v));
+                        sum = fmaf(query[group * kRowsEach + i], Y[i], sum);
+                    }
+                }
+                if (t < p0) continue;
+                sums[group][col] = sum;
+                __syncthreads();
+                if (tid < cols && out_is_nan(t, tid)) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int g = 0; g < kThreads / kSlab; ++g) x += sums[g][tid];
+                    const long long at = out0 + (long long)t * r.o.st + (long long)tid * r.o.sd;
+                    if (r.out_f32)
+                        o32[at] = x;
+                    else
+                        o16[at] = E::from_float(x);
+                }
+            }
+        }
+    }
+}
+
+}  // namespace
+}  // namespace lin
+
+cudaError_t launch_linear_isolate(const lin::Launch& l, int dtype, cudaStream_t s) {
+    using namespace lin;
+    int slabs = 0;
+    for (int i = 0; i < l.runs; ++i) slabs = max(slabs, (l.run[i].dv + kSlab - 1) / kSlab);
+    const int pieces = l.c.batch * l.c.heads * slabs;  // fits: checked with the arguments
+    // a programmatic dependent of the main kernel: its launch does not wait for that one to drain
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((l.c.seqlen + kPart - 1) / kPart, pieces < 65535 ? pieces : 65535, l.runs);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    switch (dtype) {
+        case VC1D_F32: return cudaLaunchKernelEx(&cfg, k_linear_isolate<VC1D_F32>, l, pieces, slabs);
+        case VC1D_BF16: return cudaLaunchKernelEx(&cfg, k_linear_isolate<VC1D_BF16>, l, pieces, slabs);
+        default: return cudaLaunchKernelEx(&cfg, k_linear_isolate<VC1D_F16>, l, pieces, slabs);
+    }
+}
+
+}  // namespace vc1d

@@ -271,8 +271,8 @@ def linear_attention_fn(
         dtype (float32, bfloat16, float16), any strides (parts of one fused projection too).  ``heads_k`` and ``heads_v``
         divide ``heads``; head h reads key head ``h // (heads // heads_k)``, likewise for v.  Dims 1..256.
       log_decay ``[heads]`` float32, fixed (no gradient), usually negative; 0 never forgets, ``-inf`` keeps one token.
-      seq_idx ``[batch, seqlen]`` (int32): packed rows; the state starts at zero wherever the value changes.  Not
-        combined with a mask or states, as in ``causal_conv1d_fn``.
+      seq_idx ``[batch, seqlen]`` (int32): packed rows; the state starts at zero wherever the value changes, and an infinity
+        or NaN of one sequence does not reach another.  Not combined with a mask or states, as in ``causal_conv1d_fn``.
       initial_states fp32 ``[batch, heads, dim_k, dim_v]``: continues a prompt.  ``return_final_states`` /
         ``final_states_out`` give the state that the next part or ``linear_attention_update`` continues from (it must not
         overlap ``initial_states``).

@@ -161,3 +161,20 @@ def test_new_forms_are_remembered_after_hundreds_of_others(monkeypatch):
             assert checked == (["_fill", "_check_heads", "_check_heads"] if turn == 0 else []), (n, turn)
             checked.clear()
     assert len(la._prepared("linear_args")) <= 256 and len(la._prepared("linear_update_args")) <= 256
+
+
+@pytest.mark.parametrize("kernel", ["simt", "mma", "tc"])
+def test_gradients_that_arrive_expanded(kernel):
+    """The gradient of a sum is one value, repeated by strides of 0, which the named tensor-core kernels do not take."""
+    q, k, v, *_ = (x.to(DEV) for x in make(1, 150, 2, 2, 2, 64, 64, torch.bfloat16))
+    g = decays(2).to(DEV)
+    grads = []
+    for whole in (False, True):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        o = V.linear_attention_fn(*leaves, g, kernel=kernel)
+        (o.backward(torch.ones_like(o)) if whole else o.sum().backward())
+        grads.append([x.grad for x in leaves])
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    torch.compile(lambda *x: V.linear_attention_fn(*x, g, kernel=kernel).sum(), backend="aot_eager")(*leaves).backward()
+    grads.append([x.grad for x in leaves])
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(*grads))

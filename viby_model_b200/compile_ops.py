@@ -189,6 +189,8 @@ def _linear_setup(ctx, inputs, output):
 
 def _linear_backward(ctx, dout, dstate):
     q, k, v, log_decay, seq_idx, init, mask = ctx.saved_tensors
+    if ctx.kernel != "auto":  # the kernel that the caller named may not take every layout
+        dout = dout.contiguous()
     dq, dk, dv, dinit = torch.ops.vc1d.linear_attention_bwd(q, k, v, log_decay, dout, seq_idx, init,
                                                             dstate if ctx.want_state else None, mask, ctx.scale, ctx.kernel, ctx.segments)
     return dq, dk, dv, None, None, dinit if init is not None else None, None, None, None, None, None

@@ -392,6 +392,8 @@ class _LinearAttentionFunction(torch.autograd.Function):
             return (None,) * 11
         if dout is None:
             dout = q.new_zeros(1).expand(*q.shape[:3], v.shape[3])
+        if ctx.kernel not in (None, "auto"):  # the kernel that the caller named may not take every layout
+            dout = dout.contiguous()
         if dstate is not None and dstate.numel() == 0 and v.shape[0] > 0:
             dstate = None  # no final state was returned
         grads = linear_attention_bwd(q, k, v, log_decay, dout, seq_idx, init, dstate, attention_mask=mask, scale=ctx.scale,

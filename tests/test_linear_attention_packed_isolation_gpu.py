@@ -112,3 +112,36 @@ def test_captured_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.isfinite(o).all() and torch.equal(o[:, 128:], want[:, 128:])
+
+
+@pytest.mark.parametrize("dtype,kernel,D", [("bf16", "tc", 64), ("bf16", "tc", 160), ("bf16", "mma", 128), ("f16", "mma", 64), ("f32", "simt", 40)])
+@pytest.mark.parametrize("seed", range(8))
+def test_random_lengths_and_places(dtype, kernel, D, seed):
+    """Outputs and gradients of every token that a bad value must not reach are what they are without it (within the roundings of
+    another way to compute them)."""
+    dt, H = DTYPES[dtype], 2
+    r = torch.Generator().manual_seed(100 + seed)
+    lengths = []
+    while sum(lengths) < 700:
+        lengths.append(int(torch.randint(1, (6, 60, 300)[seed % 3], (1,), generator=r)))
+    n = sum(lengths)
+    q, k, v, do, *_ = make(1, n, H, 1, H, D, D, dt, seed)
+    g = dev(decays(H))
+    seq = dev(V.seq_idx_from_lengths(lengths))
+    ids = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
+    args = dict(kernel=kernel, segments=1 + seed % 3)
+    want = (V.linear_attention_fn(dev(q), dev(k), dev(v), g, seq, **args), *V.linear_attention_bwd(dev(q), dev(k), dev(v), g, dev(do), seq, **args)[:3])
+    M = magnitudes(q, k, v, g.cpu(), seq_idx=seq.cpu())[0], *grad_magnitudes(q, k, v, g.cpu(), do, seq_idx=seq.cpu())[:3]
+    before, after = torch.ones(n, dtype=torch.bool), torch.ones(n, dtype=torch.bool)
+    for _ in range(int(torch.randint(1, 4, (1,), generator=r))):
+        t = int(torch.randint(0, n, (1,), generator=r))
+        x = (q, k, v, do)[int(torch.randint(0, 4, (1,), generator=r))]
+        x[0, t, int(torch.randint(0, x.shape[2], (1,), generator=r)), int(torch.randint(0, D, (1,), generator=r))] = (float("inf"), float("nan"))[seed % 2]
+        same = ids == ids[t]
+        before &= ~(same & (torch.arange(n) >= t))
+        after &= ~(same & (torch.arange(n) <= t))
+    got = (V.linear_attention_fn(dev(q), dev(k), dev(v), g, seq, **args), *V.linear_attention_bwd(dev(q), dev(k), dev(v), g, dev(do), seq, **args)[:3])
+    for x, w, m, clean, name in zip(got, want, M, (before, before, after, after), ("out", "dq", "dk", "dv")):
+        w = w.cpu().double()
+        tol = 2 * tolerance(w, m, dt, D + H, n, kernel != "simt")  # of either way
+        check(x[:, dev(clean)], w[:, clean], tol[:, clean], f"{name}, {lengths}")

@@ -8,10 +8,13 @@
 //     Y_t = a Y_{t-1} + s k_t v_t^T,   o_t = q_t^T Y_t     from the sequence's first token,
 // and replaces the NaN.  All other outputs stay as they are.
 //
-// Bound by its launch and by reading the outputs.  A CTA takes 256 tokens of one (row, head, slab of 64 columns).  24567 tokens
-// of 8 heads of 64 in fp16, 25 MB: 10 us behind a main kernel of 102; 300 tokens: 3 us.  Registers for two CTAs an SM: with
-// four or six the clean case takes the same time, and the recurrence, which costs about a microsecond a token and runs
-// only behind a neighbour's bad value, spills.
+// It need not read all outputs.  A bad value in a chunk shows in the chunk's last token (as an infinity where that is of the same
+// sequence, else as the NaN that 0 times it is), a bad state in all tokens of the sequence that the chunk starts in: the
+// last token of every 64 (both lengths of chunks end there) and of every sequence tell.
+//
+// Bound by its launch and its latency.  A CTA takes 256 tokens of one (row, head, slab of 64 columns).  24567 tokens of 8 heads of
+// 64: 6 us (bf16) to 10 us (fp16) behind main kernels of 81 and 102; 300 tokens: 3 us.  1024 tokens a CTA, or more CTAs an SM
+// for fewer registers, took the same.  The recurrence costs about a microsecond a token, behind a neighbour's bad value only.
 #include "linear_attention.cuh"
 
 namespace vc1d {
@@ -74,11 +77,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_isolate(const __grid_con
         const long long out0 = (long long)b * r.o.sb + (long long)h * r.o.sh + (long long)c0 * r.o.sd;
         float* o32 = static_cast<float*>(const_cast<void*>(r.o.p));
         T* o16 = static_cast<T*>(const_cast<void*>(r.o.p));
-        auto out_is_nan = [&](int i, int col) {
+        auto output = [&](int i, int col) {
             const long long at = out0 + (long long)i * r.o.st + (long long)col * r.o.sd;
-            const float x = r.out_f32 ? o32[at] : E::to_float(o16[at]);
-            return x != x;
+            return r.out_f32 ? o32[at] : E::to_float(o16[at]);
         };
+        auto out_is_nan = [&](int i, int col) { return is_nan(output(i, col)); };
         // whether any output of the tokens first .. last - 1 is NaN; one answer for the CTA
         auto nan_among = [&](int first, int last) {
             bool bad = false;
@@ -89,14 +92,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_isolate(const __grid_con
             }
             return __syncthreads_or(bad) != 0;
         };
-        if (!nan_among(i0, i1)) continue;
-
         auto starts = [&](int i) {  // whether a sequence starts at token i
             if (i == 0) return true;
             const long long at = r.reverse ? c.seqlen - 1 - i : i;
             const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + at * c.seq_st;
             return p[0] != (r.reverse ? p[c.seq_st] : p[-c.seq_st]);
         };
+        {
+            const int i = i0 + tid, lane = tid & 31;
+            unsigned tell = __ballot_sync(0xffffffffu, i < i1 && ((i & (kChunk - 1)) == kChunk - 1 || i == c.seqlen - 1 || starts(i + 1)));
+            bool bad = false;
+            while (tell != 0) {  // four tokens' rows at once
+                float x[4][2];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const int t = tell != 0 ? i - lane + __ffs(tell) - 1 : -1;
+                    tell &= tell - 1;
+                    x[n][0] = t >= 0 && lane < cols ? output(t, lane) : 0.f;
+                    x[n][1] = t >= 0 && lane + 32 < cols ? output(t, lane + 32) : 0.f;
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) bad |= !isfinite(x[n][0]) | !isfinite(x[n][1]);
+            }
+            if (!__syncthreads_or(bad) || !nan_among(i0, i1)) continue;
+        }
         for (int p0 = i0, p1; p0 < i1; p0 = p1) {  // the sequences of the part
             __syncthreads();
             if (tid == 0) found = i1;

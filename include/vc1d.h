@@ -334,7 +334,7 @@ VC1D_API uint32_t vc1d_sizeof_update_bwd_args(void);
  * companion of the Canon convolution; the reference's attention (model/model.py:760-900) is a softmax over a growing
  * cache, so it has no counterpart there.  With a = exp(log_decay[h]):
  *     valid token:   S_t = a S_{t-1} + k_t v_t^T,   o_t = scale * q_t^T S_t
- *     masked token:  S_t = S_{t-1},                 o_t = 0      (its q, k, v are not read)
+ *     masked token:  S_t = S_{t-1},                 o_t = 0      (whatever its q, k, v hold)
  *     packed rows:   S starts at zero at the first token of each run of equal seq_idx
  * An infinity or NaN of a valid token may reach earlier tokens of its row in the same chunk (64 or 128 tokens) as NaN; in
  * packed rows it stays in its sequence, behind the token that has it.

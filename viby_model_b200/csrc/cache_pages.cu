@@ -9,8 +9,8 @@
 // Every CTA works out the list of moves by itself from the index arrays (a few hundred entries, from L2) and then walks
 // strips; that is cheaper than a launch of its own for the plan.
 //
-// Measured: compacting half of 512 pages of 6 layers of linear attention states of 4 heads of 160 x 160 in 125 us (5.0 TB/s,
-// 0.77 of a plain copy's rate); small moves are latency: three pages of 18 such layers forked in 10 us.
+// Measured: compacting half of 512 pages of 6 layers of linear attention states of 4 heads of 160 x 160 in 122 to 133 us (4.7
+// to 5.1 TB/s, 0.72 to 0.78 of a plain copy's rate); small moves are latency: three pages of 18 such layers forked in 10 us.
 #include <algorithm>
 
 #include "vc1d_common.cuh"

@@ -229,7 +229,9 @@ int plan_launch(const Launch& l, int dtype, int kernel, int wanted) {
     int n = wanted;
     if (n == 0) {
         // Time in units of a chunk: waves of CTAs, each of them its chunks and a start-up of one and a half; a split adds
-        // the pass over keys and values that finds the parts' states (0.4 of a chunk's work) and the join.
+        // the pass over keys and values that finds the parts' states (0.4 of a chunk's work) and the join.  Against 15 other
+        // counts from 1 to 64 the choice is the fastest or within 1 % of it for nine shapes of all kernels (1000 to 24567 tokens
+        // on the tensor cores, 777 and 4000 in fp32), and 2 % behind for 65536 tokens of 16 heads of 128 (619 us, 605 with 4).
         const long long slots = (long long)ctas_per_sm(l, kind) * sm_count();
         double best = 0;
         for (int m = 1; m <= std::min(kMaxSegments, std::max(1, chunks)); ++m) {

@@ -15,9 +15,15 @@
 // Roundings.  The state that the queries read and the products inside a chunk are rounded to the I/O type, as operands
 // of the second product: each term of an output meets one such rounding, of the size of the output's own.  The state
 // itself is fp32 in every respect: the weighted keys are split into three bf16 parts (24 bits), fp16 ones into two tf32
-// parts (22 bits, and no trouble with fp16's range), and a chunk's sum is formed from zero and then added to the state, because the tensor cores truncate where an fp32 add rounds: thousands of
-// accumulations onto one long-lived state would all err towards zero.
-// fp16's range: the rounded state and the products are scaled by powers of two (per CTA, per query) around their maximum.
+// parts (22 bits, and no trouble with fp16's range), and a chunk's sum is formed from zero and then added to the state,
+// because the tensor cores truncate where an fp32 add rounds: thousands of accumulations onto one long-lived state would
+// all err towards zero.  fp16's range: the rounded state and the products are scaled by powers of two (per CTA, per query)
+// around their maximum.
+//
+// What bounds it: mma.sync itself, and the parts of the state's products.  8 x 1024 tokens of 16 heads of 128: 123 us in bf16,
+// 143 us in fp16 (tcgen05, bf16: 64).  Spills, all of them small (bytes stored, bf16 / fp16): 160 x 80 rows 360 / 236, 256
+// rows 96 / 108, 128 rows 20 / 132; those of 256 rows come from the test for chunks without a token: 1 to 2 % for dense
+// prompts, while padded ones are 2 to 5 % faster by it.
 #pragma once
 
 #include "linear_attention.cuh"
@@ -29,6 +35,7 @@ namespace mma {
 constexpr int kWarps = 4;             // of each kind
 constexpr int kThreads = 2 * 32 * kWarps;
 constexpr int kPad = 8;               // zeros before the table of decays of pairs
+constexpr int kSms = 148;             // of a B200; with another count the schedulers' loads are less even, no more
 
 struct Info {  // of a chunk's tokens, by one warp two chunks ahead
     float carry[kChunk];   // a^{n_i} for tokens of the sequence that the chunk starts in, else 0
@@ -251,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, DAP == 256 ? 1 : 2) k_linear_mma(con
         if constexpr (Registers<DAP>::kShares) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers<DAP>::kOut));
         // The later a warp's queries are, the more keys they see.  Every other wave of CTAs deals the 16-row groups out in
         // reverse, so that the two CTAs of an SM load its four schedulers alike.
-        const int grp = ((blockIdx.x / 148) & 1) ? kWarps - 1 - warp : warp;
+        const int grp = ((blockIdx.x / kSms) & 1) ? kWarps - 1 - warp : warp;
         T* sq = sm + L::kQ + grp * 16 * L::kStrideA;  // this warp's rows of q
         auto load_q = [&](int chunk) {
             const Info* f = infos + chunk % 3;

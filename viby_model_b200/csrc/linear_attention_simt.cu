@@ -6,7 +6,7 @@
 // is a register tile of 4 x 4 outputs per thread, fed by 128-bit shared loads (8 of them per 64 multiply-adds).
 //
 // Bound by those shared loads and by latency: a forward and backward pass over 3 x 777 tokens of 6 heads of 72 and 88 takes
-// 430 us in fp32, where memory would allow 2.5: 18 (row, head) pairs and two slabs for 148 SMs, so that the time axis is split
+// 410 us in fp32, where memory would allow 2.5: 18 (row, head) pairs and two slabs for 148 SMs, so that the time axis is split
 // and every part computed twice over, once for its state.
 #include "linear_attention.cuh"
 

@@ -24,12 +24,14 @@
 //
 // What bounds it: shared memory and the chain of a chunk.  A chunk of 128 state rows moves some 440 KB through shared memory
 // (KV reads k^T three times, once for each part), 3400 cycles of the 5300 that a chunk takes; with 160 rows it is 620 KB,
-// 4900 of 7200 to 9000.  The tensor cores work for less than a third of the time, HBM for a sixth.  8 x 1024 tokens of 16
-// heads of 128: 79 us (the warp-level kernel: 134); 64 x 1024 of 4 heads of 128: 128 us, of 160: 247 us; 65536 tokens of
-// 16 heads of 128: 641 us, 0.25 of the rate that memory would allow.
+// 4900 of 7200 to 9000.  The tensor cores work for less than a third of the time, HBM for a sixth.  Launches of a captured
+// graph: 8 x 1024 tokens of 16 heads of 128 64 us (the warp-level kernel: 123); 64 x 1024 of 4 heads of 128 118 us, of 160
+// 224 us; 65536 tokens of 16 heads of 128, three launches, 620 us, 0.26 of the rate that memory would allow.  80 registers
+// a thread leave spills of 88 bytes (128 rows) and 184 (160 rows), none where only states are wanted.
 // Measured and not taken: a second warp that issues products, weighing in two halves, a second buffer of keys for 160
-// rows (their last 32 channels as half a panel).  Together they gave 608 us for the last of these, but a training step of
-// padded rows of 160 took 1060 us instead of 1005, because the warp that clears masked rows then also asks for tokens.
+// rows (their last 32 channels as half a panel).  On one and the same GPU together 631 us instead of 637 for the last of
+// these, but 1069 instead of 996 for a training step of heads of 160, because the warp that clears masked rows then also
+// asks for tokens.
 //
 // Shared memory holds every operand as panels of 64 channels: rows of 128 bytes with the 16-byte units XORed by the row
 // modulo 8 (the 128-byte swizzle of the matrix descriptors).  A panel serves as K-major (channels summed: q, k) and as

@@ -7,7 +7,7 @@
 // the rows of S is finished with shuffles and one exchange through shared memory.
 //
 // Measured: 256 requests of 16 heads of 128 x 128 in 100 us (5.3 TB/s, 0.80 of a plain copy's rate, which is what a read
-// and write of the same lines reaches here); one request of 4 heads of 160 x 160 in 3.6 us, which is launch and latency.
+// and write of the same lines reaches here); one request of 4 heads of 160 x 160 in 4 us, which is launch and latency.
 #include "linear_attention.cuh"
 
 namespace vc1d {

@@ -276,8 +276,8 @@ def linear_attention_fn(
       initial_states fp32 ``[batch, heads, dim_k, dim_v]``: continues a prompt.  ``return_final_states`` /
         ``final_states_out`` give the state that the next part or ``linear_attention_update`` continues from (it must not
         overlap ``initial_states``).
-      attention_mask ``[batch, seqlen]`` (bool / int / float; nonzero = valid): a masked token is not read, leaves the state
-        as it is (no decay either) and its output is 0.
+      attention_mask ``[batch, seqlen]`` (bool / int / float; nonzero = valid): a masked token has no effect whatever it holds,
+        leaves the state as it is (no decay either) and its output is 0.
       scale: a number, ``dim_k ** -0.5`` by default.
       kernel: None, "simt", "mma" or "tc".  16-bit inputs go to the tensor cores by default, where the products inside a chunk
         and the state that queries read are rounded to 16 bits before the second product; "simt" keeps both in fp32, at the

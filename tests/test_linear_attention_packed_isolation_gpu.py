@@ -145,3 +145,28 @@ def test_random_lengths_and_places(dtype, kernel, D, seed):
         w = w.cpu().double()
         tol = 2 * tolerance(w, m, dt, D + H, n, kernel != "simt")  # of either way
         check(x[:, dev(clean)], w[:, clean], tol[:, clean], f"{name}, {lengths}")
+
+
+@pytest.mark.parametrize("dtype,kernel,D", [("bf16", "tc", 64), ("bf16", "mma", 64), ("f16", "mma", 160), ("f32", "simt", 40)])
+@pytest.mark.parametrize("places", [[("v", 1)], [("v", 1), ("v", 700)], [("k", 2), ("q", 255), ("q", 256)], [("k", 2), ("q", 255), ("v", 300)],
+                                    [("q", 255), ("v", 300)], [("q", 255), ("q", 256), ("v", 257)], [("q", 511), ("k", 512), ("v", 1020)],
+                                    [("v", 1002), ("k", 1044)], [("v", 1003), ("v", 1342)], [("q", 767), ("v", 1002), ("k", 1030)]])
+def test_bad_values_at_the_borders_of_parts(dtype, kernel, D, places):
+    """Sequences over several parts of 256 tokens: one part repairs what a bad state did to the others, each what is its own."""
+    dt, H, lengths = DTYPES[dtype], 2, [3, 1000, 40, 300]
+    n = sum(lengths)
+    q, k, v, *_ = make(1, n, H, H, H, D, D, dt, 11)
+    g = decays(H, "none" if D == 64 else "mixed")
+    seq = V.seq_idx_from_lengths(lengths)
+    ref, _ = O.linear_attention(q, k, v, g, seq_idx=seq)
+    M, _ = magnitudes(q, k, v, g, seq_idx=seq)
+    clean = torch.ones(n, dtype=torch.bool)
+    for what, at in places:
+        {"q": q, "k": k, "v": v}[what][0, at, :, 3] = float("inf")
+        if what == "q":
+            clean[at] = False
+        else:
+            clean[(seq[0] == seq[0, at]) & (torch.arange(n) >= at)] = False
+    for segments in (1, 2):
+        o = V.linear_attention_fn(dev(q), dev(k), dev(v), dev(g), dev(seq), kernel=kernel, segments=segments)
+        check(o[:, dev(clean)], ref[:, clean], tolerance(ref, M, dt, D, n, kernel != "simt")[:, clean], str(places))

@@ -14,7 +14,7 @@
 //
 // Bound by its launch and its latency.  A CTA takes 256 tokens of one (row, head, slab of 64 columns).  24567 tokens of 8 heads of
 // 64: 6 us (bf16) to 10 us (fp16) behind main kernels of 81 and 102; 300 tokens: 3 us.  1024 tokens a CTA, or more CTAs an SM
-// for fewer registers, took the same.  The recurrence costs about a microsecond a token, behind a neighbour's bad value only.
+// for fewer registers, took the same.  The recurrence costs about two microseconds a token, behind a bad value only.
 #include "linear_attention.cuh"
 
 namespace vc1d {
@@ -24,7 +24,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPart = kThreads;  // tokens of a CTA
 constexpr int kSlab = 64;
-constexpr int kRowsEach = kMaxDim / (kThreads / kSlab);  // state rows of a thread
+constexpr int kGroups = kThreads / kSlab;
+constexpr int kRowsEach = kMaxDim / kGroups;  // state rows of a thread
 
 __device__ __forceinline__ bool is_nan(float x) { return x != x; }
 __device__ __forceinline__ bool is_nan(__nv_bfloat16 x) { return (__bfloat16_as_ushort(x) & 0x7fffu) > 0x7f80u; }
@@ -59,7 +60,7 @@ template <int DT>
 __global__ void __launch_bounds__(kThreads, 2) k_linear_isolate(const __grid_constant__ Launch l, int pieces, int slabs_most) {
     using E = Elem<DT>;
     using T = typename E::type;
-    __shared__ float key[kMaxDim], query[kMaxDim], sums[kThreads / kSlab][kSlab];
+    __shared__ float key[kMaxDim], query[kMaxDim], sums[kGroups][kSlab];
     __shared__ int found;
     griddep_wait();
     const Run& r = l.run[blockIdx.z];
@@ -135,19 +136,24 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_isolate(const __grid_con
                 first = found;
                 if (first >= 0) break;
             }
+            // A bad state is in every token of the sequence from there on.  The part where that begins goes on through the others
+            // (below): one walk for each sequence, however long.
+            if (first < i0 && nan_among(i0 - 1, i0) && nan_among(i0, i0 + 1)) continue;
             // the sequence's first token with a key, or a value of this slab, that is not finite
             int end = p1;
-            for (int t0 = first; t0 < p1 && end == p1; t0 += kThreads / 32) {
-                const int t = t0 + (tid >> 5);
-                bool bad = false;
-                if (t < p1) {
-                    for (int d = tid & 31; d < r.da; d += 32) bad = bad || !isfinite(E::to_float(pk[(long long)t * r.k.st + d * r.k.sd]));
-                    for (int d = tid & 31; d < cols; d += 32) bad = bad || !isfinite(E::to_float(pv[(long long)t * r.v.st + d * r.v.sd]));
+            // (a token a warp at first: where all is bad that is enough)
+            for (int t0 = first, each = 1; t0 < p1 && end == p1; t0 += kThreads / 32 * each, each = 32) {
+                int worst = p1;
+                for (int t = min(p1, t0 + (tid >> 5) * each + each) - 1; t >= t0 + (tid >> 5) * each; --t) {
+                    bool bad = false;
+                    for (int d = tid & 31; d < r.da; d += 32) bad |= !isfinite(E::to_float(pk[(long long)t * r.k.st + d * r.k.sd]));
+                    for (int d = tid & 31; d < cols; d += 32) bad |= !isfinite(E::to_float(pv[(long long)t * r.v.st + d * r.v.sd]));
+                    if (bad) worst = t;
                 }
                 __syncthreads();
                 if (tid == 0) found = p1;
                 __syncthreads();
-                if (bad) atomicMin(&found, t);
+                if (worst < p1) atomicMin(&found, worst);
                 __syncthreads();
                 end = found;
             }
@@ -157,34 +163,61 @@ __global__ void __launch_bounds__(kThreads, 2) k_linear_isolate(const __grid_con
             const double e = exp((double)c.log_decay[h]);
             const float hi = (float)e, lo = isfinite(hi) ? (float)(e - (double)hi) : 0.f;
             float Y[kRowsEach] = {};
+            static_assert(kThreads == kMaxDim, "a thread per channel of a key");
+            // a token's values as they are, asked for a token ahead
+            T k_t = E::from_float(0.f), q_t = k_t, v_t = k_t, o_t = k_t;
+            float o_t32 = 0.f;
+            int id_t = 0, id_before = 0;
+            auto ask = [&](int t) {
+                if (tid < r.da) k_t = pk[(long long)t * r.k.st + tid * r.k.sd];
+                if (tid < r.da && t >= p0) q_t = pa[(long long)t * r.a.st + tid * r.a.sd];
+                if (col < cols) v_t = pv[(long long)t * r.v.st + col * r.v.sd];
+                if (t >= p0 && tid < cols) {
+                    const long long at = out0 + (long long)t * r.o.st + (long long)tid * r.o.sd;
+                    if (r.out_f32)
+                        o_t32 = o32[at];
+                    else
+                        o_t = o16[at];
+                }
+                if (t >= i1) {
+                    const int32_t* p = c.seq_idx + (long long)b * c.seq_sb + (r.reverse ? c.seqlen - 1 - t : t) * c.seq_st;
+                    id_t = p[0], id_before = r.reverse ? p[c.seq_st] : p[-c.seq_st];
+                }
+            };
+            ask(first);
             for (int t = first; t < end; ++t) {
                 __syncthreads();  // key, query and sums have been read
-                if (tid < kMaxDim) {
-                    key[tid] = tid < r.da ? E::to_float(pk[(long long)t * r.k.st + tid * r.k.sd]) : 0.f;
-                    query[tid] = tid < r.da && t >= p0 ? E::to_float(pa[(long long)t * r.a.st + tid * r.a.sd]) : 0.f;
-                }
-                __syncthreads();
-                const float v = col < cols ? E::to_float(pv[(long long)t * r.v.st + col * r.v.sd]) * r.s_pair : 0.f;
+                const float k_now = E::to_float(k_t), v_now = E::to_float(v_t), v = v_now * r.s_pair;
+                key[tid] = k_now;
+                query[tid] = E::to_float(q_t);
+                const bool replace = tid < cols && (r.out_f32 ? is_nan(o_t32) : is_nan(o_t));
+                // in the parts that follow the sequence may end or have a bad value of its own
+                if (__syncthreads_or((id_t != id_before) | !isfinite(k_now) | !isfinite(v_now))) break;
+                if (t + 1 < end) ask(t + 1);
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < kRowsEach; ++i) {
-                    if (group * kRowsEach + i < r.da) {
-                        Y[i] = fmaf(Y[i], hi, fmaf(Y[i], lo, key[group * kRowsEach + i] * v));
-                        sum = fmaf(query[group * kRowsEach + i], Y[i], sum);
-                    }
+                    const int row = i * kGroups + group;
+                    if (i % 8 == 0 && i * kGroups >= r.da) break;  // channels from r.da on are zeros
+                    Y[i] = fmaf(Y[i], hi, fmaf(Y[i], lo, key[row] * v));
+                    sum = fmaf(query[row], Y[i], sum);
                 }
                 if (t < p0) continue;
                 sums[group][col] = sum;
                 __syncthreads();
-                if (tid < cols && out_is_nan(t, tid)) {
+                if (replace) {
                     float x = 0.f;
 #pragma unroll
-                    for (int g = 0; g < kThreads / kSlab; ++g) x += sums[g][tid];
+                    for (int g = 0; g < kGroups; ++g) x += sums[g][tid];
                     const long long at = out0 + (long long)t * r.o.st + (long long)tid * r.o.sd;
                     if (r.out_f32)
                         o32[at] = x;
                     else
                         o16[at] = E::from_float(x);
+                }
+                if (t + 1 == end && end % kPart == 0 && end < c.seqlen && nan_among(end, end + 1)) {
+                    ask(end);
+                    end = min(c.seqlen, end + kPart);
                 }
             }
         }
